@@ -19,6 +19,7 @@ HXM_F32, HXM_BF16, HXM_F16 = 0, 1, 2
 
 _i64x3 = ct.c_int64 * 3
 _i64x2 = ct.c_int64 * 2
+_i64x4 = ct.c_int64 * 4
 
 
 class ScanArgs(ct.Structure):
@@ -264,6 +265,92 @@ class ChunkGemmArgs(ct.Structure):
     ]
 
 
+class LinearAttnArgs(ct.Structure):
+    _fields_ = [
+        ("struct_size", ct.c_size_t),
+        ("batch", ct.c_int32), ("seqlen", ct.c_int32), ("heads", ct.c_int32), ("dk", ct.c_int32), ("dv", ct.c_int32),
+        ("io_dtype", ct.c_int),
+        ("q", ct.c_void_p), ("q_stride", _i64x3),
+        ("k", ct.c_void_p), ("k_stride", _i64x3),
+        ("v", ct.c_void_p), ("v_stride", _i64x3),
+        ("out", ct.c_void_p), ("out_stride", _i64x3),
+        ("log_decay", ct.c_void_p), ("lengths", ct.c_void_p),
+        ("s0", ct.c_void_p), ("s0_stride", _i64x4),
+        ("sT", ct.c_void_p), ("sT_stride", _i64x4),
+        ("scale", ct.c_float),
+        ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+        ("error_flag", ct.c_void_p), ("wait_limit_cycles", ct.c_int64),
+    ]
+
+
+class LinearAttnBwdArgs(ct.Structure):
+    _fields_ = [
+        ("fwd", LinearAttnArgs),
+        ("struct_size", ct.c_size_t),
+        ("dout", ct.c_void_p), ("dout_stride", _i64x3),
+        ("dsT", ct.c_void_p), ("dsT_stride", _i64x4),
+        ("dq", ct.c_void_p), ("dk", ct.c_void_p), ("dv", ct.c_void_p), ("ds0", ct.c_void_p),
+        ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+    ]
+
+
+class LinearAttnStepArgs(ct.Structure):
+    _fields_ = [
+        ("struct_size", ct.c_size_t),
+        ("batch", ct.c_int32), ("heads", ct.c_int32), ("dk", ct.c_int32), ("dv", ct.c_int32),
+        ("io_dtype", ct.c_int),
+        ("q", ct.c_void_p), ("q_stride", _i64x2),
+        ("k", ct.c_void_p), ("k_stride", _i64x2),
+        ("v", ct.c_void_p), ("v_stride", _i64x2),
+        ("out", ct.c_void_p), ("out_stride", _i64x2),
+        ("log_decay", ct.c_void_p),
+        ("state", ct.c_void_p), ("state_stride", _i64x3),
+        ("scale", ct.c_float),
+    ]
+
+
+class QkNormRopeArgs(ct.Structure):
+    _fields_ = [
+        ("struct_size", ct.c_size_t),
+        ("batch", ct.c_int32), ("seqlen", ct.c_int32), ("heads_q", ct.c_int32), ("heads_k", ct.c_int32),
+        ("dim", ct.c_int32), ("rotary", ct.c_int32),
+        ("io_dtype", ct.c_int), ("interleaved", ct.c_int32),
+        ("q", ct.c_void_p), ("q_stride", _i64x3),
+        ("k", ct.c_void_p), ("k_stride", _i64x3),
+        ("q_weight", ct.c_void_p), ("k_weight", ct.c_void_p),
+        ("positions", ct.c_void_p), ("positions_stride", _i64x2),
+        ("rope_base", ct.c_double), ("eps", ct.c_float),
+        ("q_out", ct.c_void_p), ("q_out_stride", _i64x3),
+        ("k_out", ct.c_void_p), ("k_out_stride", _i64x3),
+    ]
+
+
+class QkNormRopeBwdArgs(ct.Structure):
+    _fields_ = [
+        ("fwd", QkNormRopeArgs),
+        ("struct_size", ct.c_size_t),
+        ("dq_out", ct.c_void_p), ("dq_out_stride", _i64x3),
+        ("dk_out", ct.c_void_p), ("dk_out_stride", _i64x3),
+        ("dq_weight", ct.c_void_p), ("dk_weight", ct.c_void_p),
+        ("workspace", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+    ]
+
+
+class SampleArgs(ct.Structure):
+    _fields_ = [
+        ("struct_size", ct.c_size_t),
+        ("rows", ct.c_int32), ("vocab", ct.c_int32),
+        ("io_dtype", ct.c_int),
+        ("logits", ct.c_void_p), ("logits_row_stride", ct.c_int64),
+        ("uniforms", ct.c_void_p),
+        ("temperature", ct.c_float), ("temperature_rows", ct.c_void_p),
+        ("top_k", ct.c_int32), ("top_k_rows", ct.c_void_p),
+        ("top_p", ct.c_float), ("top_p_rows", ct.c_void_p),
+        ("min_p", ct.c_float), ("min_p_rows", ct.c_void_p),
+        ("tokens", ct.c_void_p), ("logprob", ct.c_void_p),
+    ]
+
+
 # symbol -> (restype, argtypes)
 SYMBOLS = {
     "hxm_abi_version": (ct.c_int, []),
@@ -289,6 +376,15 @@ SYMBOLS = {
     "hxm_slstm_scan_fwd": (ct.c_int, [ct.POINTER(SlstmArgs), ct.c_void_p]),
     "hxm_causal_conv1d_fwd": (ct.c_int, [ct.POINTER(ConvArgs), ct.c_void_p]),
     "hxm_rmsnorm_fwd": (ct.c_int, [ct.POINTER(RmsnormArgs), ct.c_void_p]),
+    "hxm_linear_attn_workspace_size": (ct.c_size_t, [ct.POINTER(LinearAttnArgs)]),
+    "hxm_linear_attn_fwd": (ct.c_int, [ct.POINTER(LinearAttnArgs), ct.c_void_p]),
+    "hxm_linear_attn_bwd_workspace_size": (ct.c_size_t, [ct.POINTER(LinearAttnBwdArgs)]),
+    "hxm_linear_attn_bwd": (ct.c_int, [ct.POINTER(LinearAttnBwdArgs), ct.c_void_p]),
+    "hxm_linear_attn_step": (ct.c_int, [ct.POINTER(LinearAttnStepArgs), ct.c_void_p]),
+    "hxm_qk_norm_rope_fwd": (ct.c_int, [ct.POINTER(QkNormRopeArgs), ct.c_void_p]),
+    "hxm_qk_norm_rope_bwd_workspace_size": (ct.c_size_t, [ct.POINTER(QkNormRopeBwdArgs)]),
+    "hxm_qk_norm_rope_bwd": (ct.c_int, [ct.POINTER(QkNormRopeBwdArgs), ct.c_void_p]),
+    "hxm_sample_tokens": (ct.c_int, [ct.POINTER(SampleArgs), ct.c_void_p]),
     "hxm_mlstm_gate_prologue": (ct.c_int, [ct.POINTER(MlstmGatesArgs), ct.c_void_p]),
     "hxm_mlstm_gate_epilogue": (ct.c_int, [ct.POINTER(MlstmGatesArgs), ct.c_void_p]),
 }

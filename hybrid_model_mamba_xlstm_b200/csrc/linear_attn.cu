@@ -1,0 +1,495 @@
+// linear_attn.cu — linear attention with a constant decay per head: argument checks, dispatch, the
+// CUDA-core kernel (fp32, and bf16 shapes that the tensor-core kernel does not take) and the
+// single-token step (sm_100a).
+//
+// The reference has no such kernel; the recurrence is its mLSTM loop
+// (hybrid_xmamba/kernels/tfla/tfla_interface.py:113-137) with a constant forget gate and without
+// input gate and normalizer.
+#include "linear_attn.h"
+
+#include "capi_internal.h"
+#include "common.cuh"
+
+namespace hxm {
+namespace lattn {
+
+constexpr int kTileV = 32;  // value columns per CTA
+
+struct GenericParams {
+  Common c;
+  Problem p[3];
+};
+
+// g^n for n >= 0 from log2(g) in 64 bits: exponents reach the sequence length, where a 32-bit
+// product n * log2(g) would lose the factor's low bits.
+HXM_DEV float decay_pow(double lg2, int n) { return n == 0 ? 1.f : (float)exp2(lg2 * n); }
+
+// One CTA: (batch, head), kTileV value columns, one time segment, in chunks of C steps held in shared
+// memory as fp32.  All sums are fp32 FMAs, so fp32 inputs keep their precision; per step and head
+// that is 2 C dk + 2 C dv + 4 dk dv operations on the FP32 pipe.
+template <typename T, int C>
+__global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ GenericParams gp, int dkp, int state_only) {
+  const Common& cm = gp.c;
+  const int b = blockIdx.z % cm.batch;
+  const Problem& p = gp.p[blockIdx.z / cm.batch];
+  const int h = blockIdx.y, seg = blockIdx.x % cm.nseg, e0 = (blockIdx.x / cm.nseg) * kTileV;
+  if (e0 >= p.dv) return;
+  const int ld = dkp + 4;  // row pitch of Q, K
+  extern __shared__ __align__(16) float sh[];
+  float* Q = sh;                 // [C][ld]
+  float* K = Q + C * ld;         // [C][ld]
+  float* V = K + C * ld;         // [C][32]
+  float* W = V + C * kTileV;     // [C][32]: V times its row's weight in the state
+  float* X = W + C * kTileV;     // [dkp][32]
+  float* P = X + dkp * kTileV;   // [C][C + 4]
+  float* pw = P + C * (C + 4);   // [C + 1]: g^0 .. g^C
+  const int tid = threadIdx.x;
+  const double lg2 = (double)cm.log_decay[h] * 1.4426950408889634;
+  const int n = cm.lengths ? min(max(cm.lengths[b], 0), cm.seqlen) : cm.seqlen;
+  const int u_lo = seg * cm.seg_len, u_hi = min(n, u_lo + cm.seg_len);
+  const int is = p.reverse ? 0 : 1, fs = p.reverse ? 1 : 0;
+  for (int i = tid; i <= C; i += 256) pw[i] = decay_pow(lg2, i);
+  // the state entering the segment
+  const int nprev = state_only ? 0 : min(seg, (n + cm.seg_len - 1) / cm.seg_len);
+  const float f0 = state_only || !p.s0 ? 0.f : decay_pow(lg2, n == 0 ? 0 : u_lo + is) * p.s0_scale;
+  for (int i = tid; i < dkp * kTileV; i += 256) {
+    const int d = i / kTileV, e = e0 + i % kTileV;
+    float x = 0.f;
+    if (d < p.dk && e < p.dv) {
+      if (!state_only && p.s0) x = f0 * p.s0[b * p.s0s[0] + h * p.s0s[1] + d * p.s0s[2] + e * p.s0s[3]];
+      for (int r = 0; r < nprev; ++r)
+        x = fmaf(decay_pow(lg2, u_lo - (r + 1) * cm.seg_len),
+                 p.ws[((((int64_t)b * cm.heads + h) * (cm.nseg - 1) + r) * p.dk + d) * p.dv + e], x);
+    }
+    X[i] = x;
+  }
+  T* o = static_cast<T*>(p.o) + b * p.so[0] + h * p.so[2];
+  const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + h * p.sq[2];
+  const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2];
+  if (!state_only) {  // rows past the sequence
+    const int lo = max(n, u_lo), hi = min(cm.seqlen, u_lo + cm.seg_len);
+    for (int i = tid; i < (hi - lo) * kTileV; i += 256) {
+      const int e = e0 + i % kTileV;
+      if (e < p.dv) o[(int64_t)(lo + i / kTileV) * p.so[1] + e] = from_f32<T>(0.f);
+    }
+  }
+  const bool last_seg = n == 0 ? seg == 0 : (u_lo < n && u_hi == n);
+  for (int u0 = u_lo; u0 < u_hi; u0 += C) {
+    const int nc = min(C, u_hi - u0);
+    const bool fin = !state_only && u0 + nc == n;  // exponents of the last state in the last chunk
+    const int endexp = fin ? nc - 1 + fs : nc;
+    __syncthreads();
+    for (int i = tid; i < C * dkp; i += 256) {
+      const int r = i / dkp, d = i % dkp;
+      const bool ok = r < nc && d < p.dk;
+      const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
+      K[r * ld + d] = ok ? to_f32<T>(k[t * p.sk[1] + d]) : 0.f;
+      if (!state_only) Q[r * ld + d] = ok ? to_f32<T>(q[t * p.sq[1] + d]) : 0.f;
+    }
+    for (int i = tid; i < C * kTileV; i += 256) {
+      const int r = i / kTileV, e = e0 + i % kTileV;
+      const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
+      const float x = r < nc && e < p.dv ? to_f32<T>(v[t * p.sv[1] + e]) : 0.f;
+      V[i] = x;
+      W[i] = r < nc ? x * pw[endexp - r] : 0.f;
+    }
+    __syncthreads();
+    if (!state_only) {
+      {  // P = (q_i . k_j) g^(i-j), j <= i
+        constexpr int M = C / 16;
+        const int ty = tid / 16, tx = tid % 16;
+        float acc[M][M] = {};
+        for (int d = 0; d < dkp; d += 4) {
+          float4 a[M], c[M];
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            a[m] = *reinterpret_cast<const float4*>(Q + (ty + 16 * m) * ld + d);
+            c[m] = *reinterpret_cast<const float4*>(K + (tx + 16 * m) * ld + d);
+          }
+#pragma unroll
+          for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int j = 0; j < M; ++j)
+              acc[i][j] = fmaf(a[i].x, c[j].x, fmaf(a[i].y, c[j].y, fmaf(a[i].z, c[j].z, fmaf(a[i].w, c[j].w, acc[i][j]))));
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+          for (int j = 0; j < M; ++j) {
+            const int r = ty + 16 * i, s = tx + 16 * j;
+            P[r * (C + 4) + s] = s <= r ? acc[i][j] * pw[r - s] : 0.f;
+          }
+      }
+      __syncthreads();
+      {  // out = scale (P V + g^i Q X)
+        constexpr int N = C / 8, TPR = kTileV / N;  // columns per thread, threads per row
+        const int r = tid / TPR, c0 = (tid % TPR) * N;
+        float a[N] = {}, x[N] = {};
+        for (int j = 0; j < nc; ++j) {
+          const float w = P[r * (C + 4) + j];
+#pragma unroll
+          for (int m = 0; m < N; ++m) a[m] = fmaf(w, V[j * kTileV + c0 + m], a[m]);
+        }
+        for (int d = 0; d < p.dk; ++d) {
+          const float w = Q[r * ld + d];
+#pragma unroll
+          for (int m = 0; m < N; ++m) x[m] = fmaf(w, X[d * kTileV + c0 + m], x[m]);
+        }
+        if (r < nc) {
+          const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
+#pragma unroll
+          for (int m = 0; m < N; ++m)
+            if (e0 + c0 + m < p.dv) o[t * p.so[1] + e0 + c0 + m] = from_f32<T>(p.scale * fmaf(pw[r], x[m], a[m]));
+        }
+      }
+      __syncthreads();
+    }
+    {  // X = g^endexp X + K^T W
+      const int e = (tid % 8) * 4;
+      for (int d = tid / 8; d < dkp; d += 32) {
+        float4 x = *reinterpret_cast<float4*>(X + d * kTileV + e);
+        const float f = pw[endexp];
+        x.x *= f; x.y *= f; x.z *= f; x.w *= f;
+        for (int j = 0; j < nc; ++j) {
+          const float w = K[j * ld + d];
+          const float4 y = *reinterpret_cast<const float4*>(W + j * kTileV + e);
+          x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+        }
+        *reinterpret_cast<float4*>(X + d * kTileV + e) = x;
+      }
+    }
+  }
+  __syncthreads();
+  if (state_only) {
+    if (seg < cm.nseg - 1 && u_lo < n)
+      for (int i = tid; i < dkp * kTileV; i += 256) {
+        const int d = i / kTileV, e = e0 + i % kTileV;
+        if (d < p.dk && e < p.dv) p.ws[((((int64_t)b * cm.heads + h) * (cm.nseg - 1) + seg) * p.dk + d) * p.dv + e] = X[i];
+      }
+  } else if (p.sT && last_seg) {
+    for (int i = tid; i < dkp * kTileV; i += 256) {
+      const int d = i / kTileV, e = e0 + i % kTileV;
+      if (d < p.dk && e < p.dv) p.sT[b * p.sTs[0] + h * p.sTs[1] + d * p.sTs[2] + e * p.sTs[3]] = p.sT_scale * X[i];
+    }
+  }
+}
+
+// Rounded up so that rows stay float4-aligned.
+static int padded_dk(int dk) { return (dk + 3) / 4 * 4; }
+
+static size_t generic_smem(int C, int dkp) {
+  return sizeof(float) * ((size_t)2 * C * (dkp + 4) + 2 * C * kTileV + (size_t)dkp * kTileV + C * (C + 4) + C + 4);
+}
+
+template <typename T, int C>
+static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int tiles, bool state_only, cudaStream_t st) {
+  const size_t smem = generic_smem(C, dkp);
+  HXM_CUDA_TRY(cudaFuncSetAttribute(generic_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const dim3 grid((unsigned)(tiles * gp.c.nseg), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
+  generic_kernel<T, C><<<grid, 256, smem, st>>>(gp, dkp, state_only ? 1 : 0);
+  return check_launch("hxm_linear_attn");
+}
+
+static hxm_status launch_generic(const Common& c, const Problem* p, int np, hxm_dtype io, bool state_only, cudaStream_t st) {
+  GenericParams gp{};
+  gp.c = c;
+  int dk = 0, dv = 0;
+  for (int i = 0; i < np; ++i) {
+    gp.p[i] = p[i];
+    dk = p[i].dk > dk ? p[i].dk : dk;
+    dv = p[i].dv > dv ? p[i].dv : dv;
+  }
+  const int dkp = padded_dk(dk), tiles = (dv + kTileV - 1) / kTileV;
+  // 64-step chunks while Q, K, X of the padded dk fit the shared memory of an SM, else 32
+  if (generic_smem(64, dkp) <= 227 * 1024)
+    return io == HXM_F32 ? launch_generic_c<float, 64>(gp, np, dkp, tiles, state_only, st)
+                         : launch_generic_c<__nv_bfloat16, 64>(gp, np, dkp, tiles, state_only, st);
+  return io == HXM_F32 ? launch_generic_c<float, 32>(gp, np, dkp, tiles, state_only, st)
+                       : launch_generic_c<__nv_bfloat16, 32>(gp, np, dkp, tiles, state_only, st);
+}
+
+// ---- checks, time segments, dispatch -------------------------------------------------------------
+
+constexpr int kSMs = 148;
+
+static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Segments: the recurrence is sequential in time, so a call with fewer CTAs than SMs is cut along
+// time; every segment but the last first sums its own k v^T (pass one), the others' sums are joined
+// when a segment starts.
+static void set_segments(Common& c, int64_t ctas, int chunk) {
+  const int chunks = ceil_div(c.seqlen, chunk);
+  int64_t want = ctas > 0 ? kSMs / ctas : 1;
+  if (want > chunks / 4) want = chunks / 4;
+  if (want < 2) want = 1;
+  c.seg_len = (int)(ceil_div(chunks, want) * (int64_t)chunk);
+  c.nseg = c.seqlen > 0 ? ceil_div(c.seqlen, c.seg_len) : 1;
+}
+
+static size_t ws_floats(const Common& c, const Problem& p) {
+  return (size_t)c.batch * c.heads * (c.nseg - 1) * p.dk * p.dv;
+}
+
+static hxm_status check_args(const hxm_linear_attn_args* a, const char* who) {
+  HXM_REQUIRE(a != nullptr, "%s: args is NULL", who);
+  HXM_REQUIRE(a->struct_size == sizeof(hxm_linear_attn_args), "%s: struct_size %zu != %zu", who, a->struct_size,
+              sizeof(hxm_linear_attn_args));
+  HXM_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && a->heads >= 0 && a->dk >= 1 && a->dv >= 1,
+              "%s: bad dims B=%d L=%d H=%d dk=%d dv=%d", who, a->batch, a->seqlen, a->heads, a->dk, a->dv);
+  HXM_REQUIRE(a->io_dtype == HXM_F32 || a->io_dtype == HXM_BF16, "%s: io_dtype must be f32 or bf16", who);
+  HXM_REQUIRE_SUPPORTED(a->dk <= 512, "%s: dk %d (at most 512)", who, a->dk);
+  HXM_REQUIRE_SUPPORTED((int64_t)a->batch * 3 <= 65535 && a->heads <= 65535, "%s: batch %d (at most 21845) or heads %d (at most 65535)", who,
+                        a->batch, a->heads);
+  HXM_REQUIRE_SUPPORTED(a->seqlen <= (1 << 30), "%s: seqlen %d (at most 2^30)", who, a->seqlen);
+  HXM_REQUIRE(a->scale != 0.f && a->scale - a->scale == 0.f, "%s: scale must be finite and nonzero", who);
+  return HXM_OK;
+}
+
+static Common make_common(const hxm_linear_attn_args* a) {
+  Common c{};
+  c.batch = a->batch; c.heads = a->heads; c.seqlen = a->seqlen;
+  c.log_decay = a->log_decay; c.lengths = a->lengths;
+  c.error_flag = a->error_flag;
+  c.wait_limit = a->wait_limit_cycles != 0 ? a->wait_limit_cycles : 4000000000ll;
+  return c;
+}
+
+static Problem fwd_problem(const hxm_linear_attn_args* a) {
+  Problem p{};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->out;
+  for (int i = 0; i < 3; ++i) {
+    p.sq[i] = a->q_stride[i]; p.sk[i] = a->k_stride[i]; p.sv[i] = a->v_stride[i]; p.so[i] = a->out_stride[i];
+  }
+  p.dk = a->dk; p.dv = a->dv;
+  p.s0 = a->s0; p.sT = a->sT;
+  for (int i = 0; i < 4; ++i) { p.s0s[i] = a->s0_stride[i]; p.sTs[i] = a->sT_stride[i]; }
+  p.scale = a->scale; p.s0_scale = 1.f; p.sT_scale = 1.f;
+  return p;
+}
+
+// The gradients' three runs (see linear_attn.h): dq, dv, dk.
+static void bwd_problems(const hxm_linear_attn_bwd_args* a, Problem out[3]) {
+  const hxm_linear_attn_args& f = a->fwd;
+  const int64_t L = f.seqlen, H = f.heads;
+  auto dense = [&](int64_t s[3], int d) { s[0] = L * H * d; s[1] = H * d; s[2] = d; };
+  auto copy = [](int64_t* d, const int64_t* s, int n) { for (int i = 0; i < n; ++i) d[i] = s[i]; };
+  auto turned = [](int64_t* d, const int64_t* s) { d[0] = s[0]; d[1] = s[1]; d[2] = s[3]; d[3] = s[2]; };
+  for (int i = 0; i < 3; ++i) {
+    out[i] = Problem{};
+    out[i].scale = f.scale;
+    out[i].s0_scale = 1.f;
+    out[i].sT_scale = 1.f;
+  }
+  Problem& dq = out[0];
+  dq.q = a->dout; dq.k = f.v; dq.v = f.k; dq.o = a->dq;
+  copy(dq.sq, a->dout_stride, 3); copy(dq.sk, f.v_stride, 3); copy(dq.sv, f.k_stride, 3); dense(dq.so, f.dk);
+  dq.dk = f.dv; dq.dv = f.dk;
+  dq.s0 = f.s0; turned(dq.s0s, f.s0_stride);
+  Problem& dv = out[1];
+  dv.q = f.k; dv.k = f.q; dv.v = a->dout; dv.o = a->dv;
+  copy(dv.sq, f.k_stride, 3); copy(dv.sk, f.q_stride, 3); copy(dv.sv, a->dout_stride, 3); dense(dv.so, f.dv);
+  dv.dk = f.dk; dv.dv = f.dv; dv.reverse = 1;
+  dv.s0 = a->dsT; copy(dv.s0s, a->dsT_stride, 4); dv.s0_scale = 1.f / f.scale;
+  dv.sT = a->ds0; dv.sT_scale = f.scale;
+  dv.sTs[0] = H * f.dk * f.dv; dv.sTs[1] = (int64_t)f.dk * f.dv; dv.sTs[2] = f.dv; dv.sTs[3] = 1;
+  Problem& dk = out[2];
+  dk.q = f.v; dk.k = a->dout; dk.v = f.q; dk.o = a->dk;
+  copy(dk.sq, f.v_stride, 3); copy(dk.sk, a->dout_stride, 3); copy(dk.sv, f.q_stride, 3); dense(dk.so, f.dk);
+  dk.dk = f.dv; dk.dv = f.dk; dk.reverse = 1;
+  dk.s0 = a->dsT; turned(dk.s0s, a->dsT_stride); dk.s0_scale = 1.f / f.scale;
+}
+
+// Which kernel runs these problems, and the time segments.
+static bool plan(Common& c, const Problem* p, int np, hxm_dtype io) {
+  bool tc = true;
+  int64_t ctas = 0;
+  for (int i = 0; i < np; ++i) tc = tc && tc_ok(p[i], io);
+  for (int i = 0; i < np; ++i) ctas += (int64_t)c.batch * c.heads * ceil_div(p[i].dv, tc ? 64 : kTileV);
+  set_segments(c, ctas, 128);
+  return tc;
+}
+
+static hxm_status run(Common c, Problem* p, int np, hxm_dtype io, float* ws, size_t ws_bytes, cudaStream_t st, const char* who) {
+  const bool tc = plan(c, p, np, io);
+  size_t need = 0;
+  for (int i = 0; i < np; ++i) {
+    p[i].ws = ws + need;
+    need += ws_floats(c, p[i]);
+  }
+  HXM_REQUIRE(need == 0 || (ws && ws_bytes >= need * sizeof(float)), "%s: workspace %zu bytes < %zu", who, ws_bytes,
+              need * sizeof(float));
+  for (int pass = c.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
+    if (!tc) {
+      const hxm_status s = launch_generic(c, p, np, io, pass == 0, st);
+      if (s != HXM_OK) return s;
+      continue;
+    }
+    // runs of the same padded dk share a launch
+    Problem group[3];
+    for (int wide = 0; wide < 2; ++wide) {
+      int n = 0;
+      for (int i = 0; i < np; ++i)
+        if ((p[i].dk > 128) == (wide == 1)) group[n++] = p[i];
+      if (n) {
+        const hxm_status s = launch_tc(c, group, n, pass == 0, st);
+        if (s != HXM_OK) return s;
+      }
+    }
+  }
+  return HXM_OK;
+}
+
+// ---- single-token step -----------------------------------------------------------------------------
+
+struct StepParams {
+  int heads, dk, dv;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  int64_t sq[2], sk[2], sv[2], so[2];
+  const float* log_decay;
+  float* s;
+  int64_t ss[3];
+  float scale;
+};
+
+// S = g S + k v^T and out = scale S^T q for one token: the state is read and written once, 8 dk dv
+// bytes, which is all the time there is.  One CTA per (batch, head, 32 * VEC value columns); its
+// 8 warps share the dk rows, lane l holds VEC columns, and the warps' partial sums of the output
+// join in shared memory.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) step_kernel(const StepParams p) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int e = (blockIdx.x * 32 + lane) * VEC;
+  const float g = (float)exp2((double)p.log_decay[h] * 1.4426950408889634);
+  const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + h * p.sq[1];
+  const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[1];
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[1];
+  float* s = p.s + b * p.ss[0] + h * p.ss[1];
+  __shared__ float part[8][32 * VEC];
+  float acc[VEC] = {};
+  if (e < p.dv) {
+    float vv[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) vv[i] = to_f32<T>(v[e + i]);
+#pragma unroll 4
+    for (int d = warp; d < p.dk; d += 8) {
+      const float kd = to_f32<T>(k[d]), qd = to_f32<T>(q[d]);
+      float* row = s + d * p.ss[2] + e;
+      float x[VEC];
+      if (VEC == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row);
+      else x[0] = row[0];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        x[i] = fmaf(g, x[i], kd * vv[i]);
+        acc[i] = fmaf(qd, x[i], acc[i]);
+      }
+      if (VEC == 4) *reinterpret_cast<float4*>(row) = *reinterpret_cast<float4*>(x);
+      else row[0] = x[0];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) part[warp][lane * VEC + i] = acc[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+    const int c = blockIdx.x * 32 * VEC + i;
+    if (c < p.dv) {
+      float y = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) y += part[w][i];
+      static_cast<T*>(p.o)[b * p.so[0] + h * p.so[1] + c] = from_f32<T>(p.scale * y);
+    }
+  }
+}
+
+template <typename T>
+static hxm_status launch_step(const StepParams& p, int batch, cudaStream_t st) {
+  // 16-byte state accesses where every row allows them
+  const bool vec = p.dv % 4 == 0 && reinterpret_cast<uintptr_t>(p.s) % 16 == 0 && p.ss[0] % 4 == 0 && p.ss[1] % 4 == 0 && p.ss[2] % 4 == 0;
+  if (vec) step_kernel<T, 4><<<dim3((p.dv + 127) / 128, p.heads, batch), 256, 0, st>>>(p);
+  else step_kernel<T, 1><<<dim3((p.dv + 31) / 32, p.heads, batch), 256, 0, st>>>(p);
+  return check_launch("hxm_linear_attn_step");
+}
+
+}  // namespace lattn
+}  // namespace hxm
+
+using namespace hxm;
+using namespace hxm::lattn;
+
+extern "C" size_t hxm_linear_attn_workspace_size(const hxm_linear_attn_args* a) {
+  if (check_args(a, "hxm_linear_attn_workspace_size") != HXM_OK) return 0;
+  Common c = make_common(a);
+  const Problem p = fwd_problem(a);
+  plan(c, &p, 1, a->io_dtype);
+  return ws_floats(c, p) * sizeof(float);
+}
+
+extern "C" hxm_status hxm_linear_attn_fwd(const hxm_linear_attn_args* a, void* stream) {
+  clear_error();
+  const hxm_status s = check_args(a, "hxm_linear_attn_fwd");
+  if (s != HXM_OK) return s;
+  if (a->batch == 0 || a->heads == 0) return HXM_OK;
+  HXM_REQUIRE(a->log_decay && (a->seqlen == 0 || (a->q && a->k && a->v && a->out)), "hxm_linear_attn_fwd: NULL tensor pointer");
+  Problem p = fwd_problem(a);
+  return run(make_common(a), &p, 1, a->io_dtype, static_cast<float*>(a->workspace), a->workspace_bytes,
+             static_cast<cudaStream_t>(stream), "hxm_linear_attn_fwd");
+}
+
+static hxm_status check_bwd(const hxm_linear_attn_bwd_args* a, const char* who) {
+  HXM_REQUIRE(a != nullptr, "%s: args is NULL", who);
+  HXM_REQUIRE(a->struct_size == sizeof(hxm_linear_attn_bwd_args), "%s: struct_size %zu != %zu", who, a->struct_size,
+              sizeof(hxm_linear_attn_bwd_args));
+  const hxm_status s = check_args(&a->fwd, who);
+  if (s != HXM_OK) return s;
+  HXM_REQUIRE_SUPPORTED(a->fwd.dv <= 512, "%s: dv %d (at most 512)", who, a->fwd.dv);
+  return HXM_OK;
+}
+
+extern "C" size_t hxm_linear_attn_bwd_workspace_size(const hxm_linear_attn_bwd_args* a) {
+  if (check_bwd(a, "hxm_linear_attn_bwd_workspace_size") != HXM_OK) return 0;
+  Common c = make_common(&a->fwd);
+  Problem p[3];
+  bwd_problems(a, p);
+  plan(c, p, 3, a->fwd.io_dtype);
+  return (ws_floats(c, p[0]) + ws_floats(c, p[1]) + ws_floats(c, p[2])) * sizeof(float);
+}
+
+extern "C" hxm_status hxm_linear_attn_bwd(const hxm_linear_attn_bwd_args* a, void* stream) {
+  clear_error();
+  const hxm_status s = check_bwd(a, "hxm_linear_attn_bwd");
+  if (s != HXM_OK) return s;
+  const hxm_linear_attn_args& f = a->fwd;
+  if (f.batch == 0 || f.heads == 0) return HXM_OK;
+  HXM_REQUIRE(f.log_decay && (f.seqlen == 0 || (f.q && f.k && f.v && a->dout && a->dq && a->dk && a->dv)),
+              "hxm_linear_attn_bwd: NULL tensor pointer");
+  Problem p[3];
+  bwd_problems(a, p);
+  return run(make_common(&f), p, 3, f.io_dtype, static_cast<float*>(a->workspace), a->workspace_bytes,
+             static_cast<cudaStream_t>(stream), "hxm_linear_attn_bwd");
+}
+
+extern "C" hxm_status hxm_linear_attn_step(const hxm_linear_attn_step_args* a, void* stream) {
+  clear_error();
+  HXM_REQUIRE(a != nullptr, "hxm_linear_attn_step: args is NULL");
+  HXM_REQUIRE(a->struct_size == sizeof(hxm_linear_attn_step_args), "hxm_linear_attn_step: struct_size %zu != %zu",
+              a->struct_size, sizeof(hxm_linear_attn_step_args));
+  HXM_REQUIRE(a->batch >= 0 && a->heads >= 0 && a->dk >= 1 && a->dv >= 1, "hxm_linear_attn_step: bad dims B=%d H=%d dk=%d dv=%d",
+              a->batch, a->heads, a->dk, a->dv);
+  HXM_REQUIRE(a->io_dtype == HXM_F32 || a->io_dtype == HXM_BF16, "hxm_linear_attn_step: io_dtype must be f32 or bf16");
+  HXM_REQUIRE_SUPPORTED(a->batch <= 65535 && a->heads <= 65535, "hxm_linear_attn_step: batch %d or heads %d above 65535", a->batch, a->heads);
+  if (a->batch == 0 || a->heads == 0) return HXM_OK;
+  HXM_REQUIRE(a->q && a->k && a->v && a->out && a->state && a->log_decay, "hxm_linear_attn_step: NULL tensor pointer");
+  StepParams p{};
+  p.heads = a->heads; p.dk = a->dk; p.dv = a->dv;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->out;
+  for (int i = 0; i < 2; ++i) { p.sq[i] = a->q_stride[i]; p.sk[i] = a->k_stride[i]; p.sv[i] = a->v_stride[i]; p.so[i] = a->out_stride[i]; }
+  p.log_decay = a->log_decay; p.s = a->state;
+  for (int i = 0; i < 3; ++i) p.ss[i] = a->state_stride[i];
+  p.scale = a->scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->io_dtype == HXM_F32 ? launch_step<float>(p, a->batch, st) : launch_step<__nv_bfloat16>(p, a->batch, st);
+}

@@ -35,6 +35,23 @@ def stream_of(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """A context in which ``device`` is the current CUDA device (launches go to the current device's
+    context, whatever stream they name); free when it already is."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()
 

@@ -1,0 +1,241 @@
+"""Linear attention with a constant decay per head over the hxm C ABI.
+
+The reference has no such kernel; the recurrence is its mLSTM loop
+(hybrid_xmamba/kernels/tfla/tfla_interface.py:113-137) with a constant forget
+gate and without input gate and normalizer:
+    S_t = exp(log_decay_h) S_(t-1) + k_t v_t^T,   o_t = scale * S_t^T q_t.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+from ._common import dtype_code, on_device, ptr, require_cuda, stream_of
+
+__all__ = ["linear_attention", "linear_attention_bwd", "linear_attention_step"]
+
+
+def _check_io(who, q, k, v):
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{who}: q must be fp32 or bf16, got {q.dtype}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{who}: q, k, v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+
+
+def _scale(who, scale, dk):
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale == 0 or not math.isfinite(scale) or ctypes.c_float(scale).value == 0:
+        raise ValueError(f"{who}: scale must be finite and nonzero, got {scale}")
+    return scale
+
+
+def _decay(who, log_decay, heads):
+    if log_decay.shape != (heads,):
+        raise ValueError(f"{who}: log_decay must be ({heads},), got {tuple(log_decay.shape)}")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: log_decay is a constant; it must not require a gradient")
+    return log_decay.float().contiguous()
+
+
+def _rows(t):
+    """t (.., d) as the kernels read it: unit stride in the last dim, 16-byte aligned rows where a
+    copy can bring that about (a zero stride repeats data and stays)."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return t.contiguous()
+    e = 16 // t.element_size()
+    if t.shape[-1] % e == 0 and (t.data_ptr() % 16 or any(s % e for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _set(a, name, t, n):
+    setattr(a, name, t.data_ptr())
+    setattr(a, name + "_stride", tuple(s if m > 1 else 0 for s, m in zip(t.stride()[:n], t.shape[:n])))
+
+
+def _fill(who, q, k, v, log_decay, scale, lengths, s0, error_flag, wait_limit_cycles):
+    """(args, tensors to keep alive) of the fields that the forward and the backward share."""
+    if q.dim() != 4:
+        raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
+    bsz, L, nh, dk = q.shape
+    if k.shape != q.shape or v.shape[:-1] != q.shape[:-1] or v.dim() != 4:
+        raise ValueError(f"{who}: k must be {tuple(q.shape)} and v (B, L, H, dv), got {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_io(who, q, k, v)
+    if lengths is not None:
+        if lengths.shape != (bsz,) or lengths.is_floating_point() or lengths.dtype == torch.bool:
+            raise ValueError(f"{who}: lengths must be ({bsz},) integers")
+        if lengths.dtype != torch.int32:
+            lengths = lengths.clamp(0, L).int()
+        lengths = lengths.contiguous()
+    if s0 is not None:
+        if s0.shape != (bsz, nh, dk, v.shape[-1]):
+            raise ValueError(f"{who}: initial_state must be {(bsz, nh, dk, v.shape[-1])}, got {tuple(s0.shape)}")
+        s0 = s0.float()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    ld = _decay(who, log_decay, nh)
+    a = _lib.LinearAttnArgs()
+    a.struct_size = ctypes.sizeof(a)
+    a.batch, a.seqlen, a.heads, a.dk, a.dv = bsz, L, nh, dk, v.shape[-1]
+    a.io_dtype = dtype_code(q)
+    _set(a, "q", q, 3)
+    _set(a, "k", k, 3)
+    _set(a, "v", v, 3)
+    a.log_decay, a.lengths = ptr(ld), ptr(lengths)
+    if s0 is not None:
+        a.s0, a.s0_stride = s0.data_ptr(), s0.stride()
+    a.scale = scale
+    a.error_flag, a.wait_limit_cycles = ptr(error_flag), int(wait_limit_cycles)
+    return a, (q, k, v, ld, lengths, s0)
+
+
+def _forward(q, k, v, log_decay, scale, lengths, s0, want_state, error_flag=None, wait_limit_cycles=0):
+    who = "linear_attention"
+    dev = require_cuda(q, k, v, log_decay, lengths, s0, error_flag, who=who)
+    with on_device(dev):
+        a, keep = _fill(who, q, k, v, log_decay, scale, lengths, s0, error_flag, wait_limit_cycles)
+        out = torch.empty(a.batch, a.seqlen, a.heads, a.dv, device=dev, dtype=q.dtype)
+        _set(a, "out", out, 3)
+        sT = None
+        if want_state:
+            sT = torch.empty(a.batch, a.heads, a.dk, a.dv, device=dev, dtype=torch.float32)
+            a.sT, a.sT_stride = sT.data_ptr(), sT.stride()
+        n = int(_lib.lib().hxm_linear_attn_workspace_size(a))
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+        a.workspace, a.workspace_bytes = ptr(ws), n
+        _lib.call("hxm_linear_attn_fwd", a, stream_of(dev))
+    return out, sT
+
+
+def linear_attention_bwd(q, k, v, log_decay, dout, *, scale=None, lengths=None, initial_state=None, d_final_state=None,
+                         need_d_initial_state=None, error_flag=None, wait_limit_cycles=0):
+    """Gradients of :func:`linear_attention` for dout (B, L, H, dv) and d_final_state (B, H, dk, dv) or None.
+
+    Returns (dq, dk, dv, d_initial_state): the first three in q's dtype, the last fp32, or None unless
+    ``need_d_initial_state`` (default: with an initial_state).  They are three more runs of the same
+    recurrence, dk and dv in reversed time, so dv (the size) may be at most 512 like dk."""
+    who = "linear_attention_bwd"
+    dev = require_cuda(q, k, v, log_decay, dout, lengths, initial_state, d_final_state, error_flag, who=who)
+    if dout.shape != v.shape or dout.dtype != q.dtype:
+        raise ValueError(f"{who}: dout must be {tuple(v.shape)} {q.dtype}, got {tuple(dout.shape)} {dout.dtype}")
+    scale = _scale(who, scale, q.shape[-1])
+    if need_d_initial_state is None:
+        need_d_initial_state = initial_state is not None
+    with on_device(dev):
+        f, keep = _fill(who, q, k, v, log_decay, scale, lengths, initial_state, error_flag, wait_limit_cycles)
+        dout = _rows(dout)
+        a = _lib.LinearAttnBwdArgs()
+        a.fwd = f
+        a.struct_size = ctypes.sizeof(a)
+        _set(a, "dout", dout, 3)
+        sshape = (f.batch, f.heads, f.dk, f.dv)
+        if d_final_state is not None:
+            if d_final_state.shape != sshape:
+                raise ValueError(f"{who}: d_final_state must be {sshape}, got {tuple(d_final_state.shape)}")
+            d_final_state = d_final_state.float()
+            a.dsT, a.dsT_stride = d_final_state.data_ptr(), d_final_state.stride()
+        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        dk = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        dv = torch.empty(v.shape, device=dev, dtype=q.dtype)
+        ds0 = torch.empty(sshape, device=dev, dtype=torch.float32) if need_d_initial_state else None
+        a.dq, a.dk, a.dv, a.ds0 = ptr(dq), ptr(dk), ptr(dv), ptr(ds0)
+        n = int(_lib.lib().hxm_linear_attn_bwd_workspace_size(a))
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+        a.workspace, a.workspace_bytes = ptr(ws), n
+        _lib.call("hxm_linear_attn_bwd", a, stream_of(dev))
+    return dq, dk, dv, ds0
+
+
+class LinearAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, s0, log_decay, scale, lengths, want_state):
+        ctx.save_for_backward(q, k, v, s0, log_decay, lengths)
+        ctx.scale = scale
+        out, sT = _forward(q, k, v, log_decay, scale, lengths, s0, want_state)
+        ctx.set_materialize_grads(False)
+        return out, sT
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dsT):
+        q, k, v, s0, log_decay, lengths = ctx.saved_tensors
+        if dout is None and dsT is None:
+            return (None,) * 8
+        if dout is None:
+            dout = torch.zeros(v.shape, device=v.device, dtype=v.dtype)
+        dq, dk, dv, ds0 = linear_attention_bwd(q, k, v, log_decay, dout.to(q.dtype), scale=ctx.scale, lengths=lengths,
+                                               initial_state=s0, d_final_state=dsT,
+                                               need_d_initial_state=s0 is not None and ctx.needs_input_grad[3])
+        return dq, dk, dv, ds0 if ds0 is None else ds0.to(s0.dtype), None, None, None, None
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_state=None, return_final_state=False,
+                     error_flag=None, wait_limit_cycles=0):
+    """Linear attention over whole sequences, from and to a carried state; differentiable.
+
+    q, k (B, L, H, dk), v (B, L, H, dv): bf16 or fp32, any strides (views with a unit last stride and
+    16-byte aligned rows are read in place, zero strides too, others copied); log_decay (H,) fp32, at
+    most 0 (-inf: each step forgets all before it), a constant without a gradient; scale: default
+    dk**-0.5; lengths (B,) integers: only the first lengths[b] steps of row b count (held to
+    [0, L]), later rows of the output are zero and their inputs are never used; initial_state
+    (B, H, dk, dv).  Returns o (B, L, H, dv) in q's dtype [and the state after the last counted step,
+    fp32 (B, H, dk, dv), to continue with this function or :func:`linear_attention_step`].
+
+    dk <= 512, and dv <= 512 for gradients.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
+    dv <= 256 too) runs on the tensor cores; everything else on the FP32 pipe.  error_flag: a device int32
+    tensor set to 1 if a bounded device wait gave up (the outputs are then not valid); wait_limit_cycles:
+    that bound in SM cycles (0: about 2 s)."""
+    who = "linear_attention"
+    if q.dim() != 4:
+        raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
+    scale = _scale(who, scale, q.shape[-1])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, initial_state, log_decay)):
+        if v.shape[-1] > 512:
+            raise ValueError(f"{who}: gradients need dv <= 512, got {v.shape[-1]}")
+        _decay(who, log_decay, q.shape[2])
+        out, sT = LinearAttentionFunction.apply(q, k, v, initial_state, log_decay, scale, lengths, bool(return_final_state))
+    else:
+        out, sT = _forward(q, k, v, log_decay, scale, lengths, initial_state, return_final_state, error_flag,
+                           wait_limit_cycles)
+    return (out, sT) if return_final_state else out
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
+    """One step for every row: ``state`` (B, H, dk, dv; fp32, unit last stride) becomes
+    exp(log_decay) state + k v^T in place, and o = scale * state^T q (B, H, dv) is returned (in ``out``
+    if given).  q, k (B, H, dk), v (B, H, dv): bf16 or fp32.  Without gradients."""
+    who = "linear_attention_step"
+    dev = require_cuda(q, k, v, log_decay, state, out, who=who)
+    if q.dim() != 3:
+        raise ValueError(f"{who}: q must be (B, H, dk), got {tuple(q.shape)}")
+    bsz, nh, dk = q.shape
+    dv = v.shape[-1]
+    if k.shape != q.shape or v.dim() != 3 or v.shape[:2] != q.shape[:2]:
+        raise ValueError(f"{who}: k must be {tuple(q.shape)} and v (B, H, dv), got {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_io(who, q, k, v)
+    if state.shape != (bsz, nh, dk, dv) or state.dtype != torch.float32:
+        raise ValueError(f"{who}: state must be fp32 {(bsz, nh, dk, dv)}, got {state.dtype} {tuple(state.shape)}")
+    if (dv > 1 and state.stride(-1) != 1) or any(s == 0 for s, n in zip(state.stride(), state.shape) if n > 1):
+        raise ValueError(f"{who}: state is updated in place: it needs a unit last stride and no repeated rows")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise ValueError(f"{who}: has no gradient; use linear_attention, or torch.no_grad()")
+    scale = _scale(who, scale, dk)
+    with on_device(dev):
+        unit = lambda t: t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+        q, k, v = unit(q), unit(k), unit(v)
+        ld = _decay(who, log_decay, nh)
+        if out is None:
+            out = torch.empty(bsz, nh, dv, device=dev, dtype=q.dtype)
+        elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1):
+            raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride")
+        a = _lib.LinearAttnStepArgs()
+        a.batch, a.heads, a.dk, a.dv = bsz, nh, dk, dv
+        a.io_dtype = dtype_code(q)
+        for name, t, n in (("q", q, 2), ("k", k, 2), ("v", v, 2), ("out", out, 2), ("state", state, 3)):
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_stride", t.stride()[:n])
+        a.log_decay, a.scale = ptr(ld), scale
+        _lib.call("hxm_linear_attn_step", a, stream_of(dev))
+    return out

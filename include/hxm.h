@@ -581,6 +581,155 @@ typedef struct hxm_mlstm_gates_args {
 hxm_status hxm_mlstm_gate_prologue(const hxm_mlstm_gates_args* args, void* stream);
 hxm_status hxm_mlstm_gate_epilogue(const hxm_mlstm_gates_args* args, void* stream);
 
+/* ---- Linear attention with a constant decay per head ----------------------- */
+/* For every batch row b and head h, with g = exp(log_decay[h]):              */
+/*   S_t = g S_(t-1) + k_t v_t^T,  out_t = scale * S_t^T q_t,  t = 0 .. n-1    */
+/* from S_(-1) = s0 (zero where NULL); sT (or NULL) receives S_(n-1).  n is     */
+/* lengths[b], held to [0, seqlen], or seqlen where lengths is NULL; out rows  */
+/* n .. seqlen-1 are set to zero and the inputs' rows there are never used.   */
+/* No reference kernel: the mLSTM recurrence (kernels/tfla/tfla_interface.py:  */
+/* 113-137) with a constant forget gate and without input gate, normalizer.    */
+/* q, k: (b, t, h, dk), v, out: (b, t, h, dv) of the io dtype (bf16 / fp32)   */
+/* with unit stride in the last dim, element strides (b, t, h) given; a zero   */
+/* stride repeats the data along that dim.  log_decay (heads) fp32, <= 0       */
+/* (-inf: no memory).  s0, sT: fp32 with four element strides (b, h, dk, dv).  */
+/* dk <= 512; scale finite and nonzero.  bf16 with dk <= 256, dk and dv        */
+/* multiples of 8 and 16-byte aligned rows runs on the tensor cores.           */
+typedef struct hxm_linear_attn_args {
+  size_t struct_size;
+  int32_t batch, seqlen, heads, dk, dv;
+  hxm_dtype io_dtype;
+  const void* q;  int64_t q_stride[3];
+  const void* k;  int64_t k_stride[3];
+  const void* v;  int64_t v_stride[3];
+  void* out;      int64_t out_stride[3];
+  const float* log_decay;
+  const int32_t* lengths;
+  const float* s0; int64_t s0_stride[4];
+  float* sT;       int64_t sT_stride[4];
+  float scale;
+  void* workspace; size_t workspace_bytes;
+  int* error_flag;            /* set to 1 when a bounded device wait gave up   */
+  int64_t wait_limit_cycles;  /* 0: about 2 s                                  */
+} hxm_linear_attn_args;
+
+size_t hxm_linear_attn_workspace_size(const hxm_linear_attn_args* args);
+hxm_status hxm_linear_attn_fwd(const hxm_linear_attn_args* args, void* stream);
+
+/* Gradients of hxm_linear_attn_fwd for dout (b, t, h, dv) and dsT (b, h, dk,  */
+/* dv; NULL: zero): dq, dk, dv (dense (b, t, h, d) of the io dtype) and ds0     */
+/* (dense fp32, or NULL).  fwd.out and fwd.sT are not used.  The three passes  */
+/* are the forward recurrence with the operands exchanged, dk and dv with time */
+/* reversed, so dv (the size) is limited as dk is.                             */
+typedef struct hxm_linear_attn_bwd_args {
+  hxm_linear_attn_args fwd;
+  size_t struct_size;
+  const void* dout; int64_t dout_stride[3];
+  const float* dsT; int64_t dsT_stride[4];
+  void* dq;
+  void* dk;
+  void* dv;
+  float* ds0;
+  void* workspace; size_t workspace_bytes;
+} hxm_linear_attn_bwd_args;
+
+size_t hxm_linear_attn_bwd_workspace_size(const hxm_linear_attn_bwd_args* args);
+hxm_status hxm_linear_attn_bwd(const hxm_linear_attn_bwd_args* args, void* stream);
+
+/* One step of the same recurrence, the state (b, h, dk, dv; fp32, unit stride */
+/* in dv, element strides (b, h, dk)) updated in place.  q, k: (b, h, dk),     */
+/* v, out: (b, h, dv), element strides (b, h).                                 */
+typedef struct hxm_linear_attn_step_args {
+  size_t struct_size;
+  int32_t batch, heads, dk, dv;
+  hxm_dtype io_dtype;
+  const void* q;  int64_t q_stride[2];
+  const void* k;  int64_t k_stride[2];
+  const void* v;  int64_t v_stride[2];
+  void* out;      int64_t out_stride[2];
+  const float* log_decay;
+  float* state;   int64_t state_stride[3];
+  float scale;
+} hxm_linear_attn_step_args;
+
+hxm_status hxm_linear_attn_step(const hxm_linear_attn_step_args* args, void* stream);
+
+/* ---- RMS norms of the heads of q and k with the position rotation ---------- */
+/* For every row (b, t) and head, x one head of q or k, over its dim elements: */
+/*   y = weight * x / sqrt(mean(x^2) + eps)                                    */
+/* (RMSNorm.forward per head, layers/mlstm_block.py:113-114), then pair p <     */
+/* rotary/2 of y's first `rotary` elements (elements p and p + rotary/2, or     */
+/* 2p and 2p + 1 when interleaved) turned by positions[b, t] * base^(-2p /     */
+/* rotary), the angle formed in 64 bits.  x, out: element strides (b, t, h),   */
+/* unit stride in the last dim, fp32 / bf16 / fp16; weights fp32 (dim) or NULL */
+/* (ones); positions int64 with element strides (b, t), or NULL with rotary 0. */
+/* dim <= 1024.                                                                */
+typedef struct hxm_qk_norm_rope_args {
+  size_t struct_size;
+  int32_t batch, seqlen, heads_q, heads_k, dim, rotary;
+  hxm_dtype io_dtype;
+  int32_t interleaved;
+  const void* q; int64_t q_stride[3];
+  const void* k; int64_t k_stride[3];
+  const float* q_weight;
+  const float* k_weight;
+  const int64_t* positions; int64_t positions_stride[2];
+  double rope_base;
+  float eps;
+  void* q_out; int64_t q_out_stride[3];
+  void* k_out; int64_t k_out_stride[3];
+} hxm_qk_norm_rope_args;
+
+hxm_status hxm_qk_norm_rope_fwd(const hxm_qk_norm_rope_args* args, void* stream);
+
+/* Its gradients: q_out / k_out of `fwd` hold dL/dq, dL/dk on return; dq_out,   */
+/* dk_out are the gradients of the outputs (io dtype, element strides (b, t,   */
+/* h)); dq_weight, dk_weight (dim) fp32 or NULL.  The sums over rows go through */
+/* the workspace in a fixed order.                                             */
+typedef struct hxm_qk_norm_rope_bwd_args {
+  hxm_qk_norm_rope_args fwd;
+  size_t struct_size;
+  const void* dq_out; int64_t dq_out_stride[3];
+  const void* dk_out; int64_t dk_out_stride[3];
+  float* dq_weight;
+  float* dk_weight;
+  void* workspace; size_t workspace_bytes;
+} hxm_qk_norm_rope_bwd_args;
+
+size_t hxm_qk_norm_rope_bwd_workspace_size(const hxm_qk_norm_rope_bwd_args* args);
+hxm_status hxm_qk_norm_rope_bwd(const hxm_qk_norm_rope_bwd_args* args, void* stream);
+
+/* ---- Token sampling --------------------------------------------------------- */
+/* One token for each row of logits (rows, vocab) and its uniform number u in  */
+/* [0, 1) (models/hybrid_lm.py:238-262 samples the same way with torch calls). */
+/* With x = logit / temperature and w = exp(x - max x), formed in 64 bits:      */
+/*   top_k: the top_k largest logits stay (0, or vocab and more: all);          */
+/*   top_p: of these, sorted by falling logit, those stay before which the sum */
+/*          of w is at most top_p times the total (the first always);          */
+/*   min_p: of these, those with w >= min_p stay;                              */
+/* equal logits rank by rising token.  The token is the first of the kept ones, */
+/* in rising order, up to which the sum of w exceeds u times their total.      */
+/* temperature not above 0: the largest logit.  Logits of -inf and NaN never    */
+/* stay, +inf ones share all of the weight; a row with nothing left gives -1.   */
+/* Each setting is one value, or one per row where its pointer is not NULL.    */
+/* logprob (or NULL): log(w / total) of the token over the kept ones (0 when   */
+/* greedy, -inf where nothing is left).  vocab <= 2^18.                        */
+typedef struct hxm_sample_args {
+  size_t struct_size;
+  int32_t rows, vocab;
+  hxm_dtype io_dtype;
+  const void* logits; int64_t logits_row_stride;
+  const float* uniforms;
+  float temperature; const float* temperature_rows;
+  int32_t top_k;     const int32_t* top_k_rows;
+  float top_p;       const float* top_p_rows;
+  float min_p;       const float* min_p_rows;
+  int64_t* tokens;
+  float* logprob;
+} hxm_sample_args;
+
+hxm_status hxm_sample_tokens(const hxm_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
