@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
   const int is = p.reverse ? 0 : 1, fs = p.reverse ? 1 : 0;
   for (int i = tid; i <= C; i += 256) pw[i] = decay_pow(lg2, i);
   // the state entering the segment
-  const int nprev = state_only ? 0 : min(seg, (n + cm.seg_len - 1) / cm.seg_len);
+  const int nprev = state_only || n == 0 ? 0 : min(seg, (n + cm.seg_len - 1) / cm.seg_len);
   const float f0 = state_only || !p.s0 ? 0.f : decay_pow(lg2, n == 0 ? 0 : u_lo + is) * p.s0_scale;
   for (int i = tid; i < dkp * kTileV; i += 256) {
     const int d = i / kTileV, e = e0 + i % kTileV;
@@ -304,7 +304,7 @@ static void bwd_problems(const hxm_linear_attn_bwd_args* a, Problem out[3]) {
 static bool plan(Common& c, const Problem* p, int np, hxm_dtype io) {
   bool tc = true;
   int64_t ctas = 0;
-  for (int i = 0; i < np; ++i) tc = tc && tc_ok(p[i], io);
+  for (int i = 0; i < np; ++i) tc = tc && tc_ok(p[i], c.seqlen, io);
   for (int i = 0; i < np; ++i) ctas += (int64_t)c.batch * c.heads * ceil_div(p[i].dv, tc ? 64 : kTileV);
   set_segments(c, ctas, 128);
   return tc;

@@ -49,7 +49,7 @@ struct Common {
 };
 
 // Whether the tensor-core kernel takes this run (bf16; see linear_attn_tc.cu).
-bool tc_ok(const Problem& p, hxm_dtype io);
+bool tc_ok(const Problem& p, int seqlen, hxm_dtype io);
 // Runs np <= 3 problems of equal padded dk; state_only: the segment sums of pass one.
 hxm_status launch_tc(const Common& c, const Problem* p, int np, bool state_only, cudaStream_t st);
 
