@@ -296,11 +296,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
 #pragma unroll
       for (int blk = 0; blk < kNB; ++blk) {
         const int d = blk * 128 + row;
+        const bool first = !state_only && p.s0;
+        const float* src = first ? p.s0 + b * p.s0s[0] + h * p.s0s[1] + d * p.s0s[2] + (e0 + cb) * p.s0s[3] : nullptr;
+        const bool vec = first && p.s0s[3] == 1 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int e = e0 + cb + j;
-          X[blk][j] = !state_only && p.s0 && d < p.dk && e < p.dv
-                          ? f0 * p.s0[b * p.s0s[0] + h * p.s0s[1] + d * p.s0s[2] + e * p.s0s[3]] : 0.f;
+        for (int j = 0; j < 16; j += 4) {
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (first && d < p.dk && e0 + cb + j < p.dv) {  // dv is a multiple of 8
+            if (vec) y = *reinterpret_cast<const float4*>(src + j);
+            else y = make_float4(src[j * p.s0s[3]], src[(j + 1) * p.s0s[3]], src[(j + 2) * p.s0s[3]], src[(j + 3) * p.s0s[3]]);
+          }
+          X[blk][j] = f0 * y.x;
+          X[blk][j + 1] = f0 * y.y;
+          X[blk][j + 2] = f0 * y.z;
+          X[blk][j + 3] = f0 * y.w;
         }
       }
       if (u_lo < n)
