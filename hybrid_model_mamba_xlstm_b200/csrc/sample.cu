@@ -2,9 +2,18 @@
 // given uniform number, in one launch (sm_100a).
 //
 // Replaces the sampling of HybridLanguageModel.generate (hybrid_xmamba/models/hybrid_lm.py:238-262:
-// topk, sort, softmax, cumsum, multinomial) without a sort: the logits are read from HBM once and
-// stay in shared memory as order-preserving 32-bit keys, one thread-block cluster per row; the top-k
-// and top-p borders are found by radix selection (8 bits of the key a pass) over counts and weights.
+// topk, sort, softmax, cumsum, multinomial) without a sort of the vocabulary.  One thread-block
+// cluster takes a row: the logits are read from HBM once and stay in shared memory as order-preserving
+// keys (16 bits for 16-bit logits).  What is left is a chain of passes over shared memory, and the
+// number of passes and of 64-bit exponentials in them is the cost:
+//   - counts of the logits in 4096 bins, 1/128 of exp's unit wide, below the largest one;
+//   - top_k up to 512: the tokens of the bins that hold the k largest (a few more than k) go to a list,
+//     which alone is ranked, cut and drawn from;
+//   - top_p: bin counts bound the weight above every bin from both sides to 1 part in 100, so the
+//     border lies in a few bins; one pass sums all weights and those before these bins.  The tokens of
+//     the bins are listed and ranked, after counting them once more in 4096 finer bins where they are
+//     more than 1024;
+//   - anything else (a border among more than 1024 tokens): radix selection, 8 bits of the key a pass.
 //
 // Weights w = exp((logit - max) / temperature) are formed in 64 bits and held as integers of 2^-44:
 // their sums are exact, so no order of additions (atomics, cluster size) changes a result, and a
@@ -20,10 +29,14 @@ namespace cg = cooperative_groups;
 namespace hxm {
 namespace sample {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr double kOne = 17592186044416.0;  // 2^44
 constexpr int kMaxVocab = 1 << 18;
+constexpr int kBins = 4096;
+constexpr float kBinsPerUnit = 128.f;  // 32 units in all: weights behind them are below 2^-46
+constexpr int kList = 1024;      // tokens ranked one by one
+constexpr int kTopKList = 512;   // top_k up to which the kept tokens are listed
+constexpr int kSubs = 4 * kWarps;  // runs of tokens whose weights are summed apart
 typedef unsigned long long u64;
 
 struct Params {
@@ -44,95 +57,174 @@ struct Params {
 };
 
 // Keys rise with the logit; 0 marks a masked one (-inf, NaN), so that real keys start above it.
-HXM_DEV uint32_t key_of(float x) {
-  if (!(x > -INFINITY)) return 0u;
-  const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);  // -0 and 0 are one logit
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-HXM_DEV float logit_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// -0 and 0 are one logit.
+template <typename T> struct Key;
+template <> struct Key<float> {
+  typedef uint32_t type;
+  static constexpr int kBits = 32;
+  static HXM_DEV uint32_t make(float x) {
+    if (!(x > -INFINITY)) return 0u;
+    const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+  }
+  static HXM_DEV float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+};
+template <typename T> struct Key16 {
+  typedef uint16_t type;
+  static constexpr int kBits = 16;
+  static HXM_DEV uint32_t make(T x) {
+    const float f = to_f32<T>(x);
+    if (!(f > -INFINITY)) return 0u;
+    uint32_t b = *reinterpret_cast<const uint16_t*>(&x);
+    if (f == 0.f) b = 0;
+    return b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+  }
+  static HXM_DEV float value(uint32_t k) {
+    const uint16_t b = (uint16_t)(k & 0x8000u ? k & 0x7fffu : ~k);
+    return to_f32<T>(*reinterpret_cast<const T*>(&b));
+  }
+};
+template <> struct Key<__nv_bfloat16> : Key16<__nv_bfloat16> {};
+template <> struct Key<__half> : Key16<__half> {};
 
 struct Shared {
-  u64 hist[2][256];    // this CTA's sums per bin, double-buffered between passes
-  u64 total[256];      // the cluster's
-  u64 scan[2][kWarps]; // block scans
-  u64 mine[2][2];      // this CTA's totals, double-buffered, for the cluster to read
-  uint32_t wmax[kWarps];
+  double pow2[64];  // 2^(j / 64)
+  u64 scan[kWarps];
+  u64 mine[2][2];   // this CTA's totals, double-buffered, for the cluster to read
+  u64 sub[kSubs];
+  uint32_t wred[kWarps];
+  float wredf[2][kWarps];
   uint32_t cmax;
-  int pick;
+  uint32_t cmin[1];
+  int pick, pick2;
   u64 above;
+  int run_at;
+  u64 run_sum;
+  uint32_t n_list;
+  // rank 0's verdict on a top-p border
+  uint32_t thr;
+  u64 ties;
 };
+// One region after the keys: the bins, then a list and its ranking, or the radix selection's sums.
+struct Bins { uint32_t n[kBins]; };
+struct Lists { u64 item[kList]; u64 weight[kList]; };
+struct Radix { u64 hist[2][256]; u64 total[256]; };
+constexpr size_t kRegion = sizeof(Bins);
+static_assert(sizeof(Lists) <= kRegion && sizeof(Radix) <= kRegion, "region");
 
+template <typename T>
 struct Ctx {
+  typedef typename Key<T>::type K;
   cg::cluster_group cl;
   Shared* s;
-  const uint32_t* keys;
+  unsigned char* region;
+  const K* keys;
   int n;        // this CTA's tokens
-  int e;        // tokens per thread (odd: a thread's run of keys starts in a bank of its own)
-  double max, t;
+  double max, c;  // weight of x: 2^((x - max) c)
+  float fmax, per_bin;
   uint32_t kmax;
   int flip;
 };
 
-HXM_DEV double weight_d(const Ctx& c, uint32_t key) {
-  if (key == c.kmax) return 1.0;
-  return exp(((double)logit_of(key) - c.max) / c.t);
+// 2^44 2^t for t = (x - max) log2(e) / temperature <= 0, not yet rounded to an integer: t = n / 64 + r,
+// a table for n mod 64 and the series of 2^r, whose next term is below 4e-17.  0 below 2^-46.
+template <typename T>
+HXM_DEV double weight_d(const Ctx<T>& c, uint32_t key) {
+  constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: its sum with |y| < 2^31 ends in round(y)
+  constexpr double kLn2_ = 0.69314718055994530942;
+  if (key == c.kmax) return 17592186044416.0;
+  const double t = ((double)Key<T>::value(key) - c.max) * c.c;
+  if (!(t > -46.0)) return 0.0;
+  const double z = fma(t, 64.0, kShift);
+  const int n = (int)__double2loint(z);
+  const double r = fma(z - kShift, -1.0 / 64.0, t) * kLn2_;
+  const double p = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0);
+  const double m = c.s->pow2[n & 63] * p;
+  return __hiloint2double(__double2hiint(m) + (((n >> 6) + 44) << 20), __double2loint(m));
 }
-HXM_DEV u64 weight(const Ctx& c, uint32_t key) { return (u64)__double2ll_rn(weight_d(c, key) * kOne); }
+HXM_DEV u64 to_fixed(double w) {
+  return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;  // w < 2^45: the sum's last bits
+}
+template <typename T>
+HXM_DEV u64 weight(const Ctx<T>& c, uint32_t key) { return to_fixed(weight_d(c, key)); }
 
-// Sum of v over the cluster, to every thread; `before`: over the CTAs of lower rank.
-HXM_DEV u64 cluster_sum(Ctx& c, u64 v, u64* before) {
+// Bins of falling logits: 0 next to the largest, the last one open.
+template <typename T>
+HXM_DEV int bin_of(const Ctx<T>& c, uint32_t key) {
+  if (key == c.kmax) return 0;
+  const float b = (c.fmax - Key<T>::value(key)) * c.per_bin;
+  return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+}
+
+HXM_DEV u64 warp_sum(u64 v) {
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+HXM_DEV u64 warp_prefix(u64 v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+// Inclusive sum over the block's threads up to this one.
+HXM_DEV u64 block_prefix(Shared* s, u64 v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64 a = warp_prefix(v);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) c.s->scan[0][threadIdx.x >> 5] = v;
+  if (lane == 31) s->scan[warp] = a;
   __syncthreads();
+  const u64 w = lane < warp ? s->scan[lane] : 0;
+  return a + warp_sum(w);
+}
+
+// Sums over the cluster of this CTA's values v0, v1 (same in all its threads); `before`: v0 over lower ranks.
+template <typename T>
+HXM_DEV void cluster_sum(Ctx<T>& c, u64 v0, u64 v1, u64& all0, u64& all1, u64& before) {
   if (threadIdx.x == 0) {
-    u64 a = 0;
-    for (int i = 0; i < kWarps; ++i) a += c.s->scan[0][i];
-    c.s->mine[c.flip][0] = a;
+    c.s->mine[c.flip][0] = v0;
+    c.s->mine[c.flip][1] = v1;
   }
   c.cl.sync();
-  u64 all = 0, pre = 0;
+  all0 = all1 = before = 0;
   for (unsigned r = 0; r < c.cl.num_blocks(); ++r) {
-    const u64 x = c.cl.map_shared_rank(&c.s->mine[c.flip][0], r)[0];
-    if (r < c.cl.block_rank()) pre += x;
-    all += x;
+    const u64* m = c.cl.map_shared_rank(&c.s->mine[c.flip][0], r);
+    const u64 x = m[0];
+    if (r < c.cl.block_rank()) before += x;
+    all0 += x;
+    all1 += m[1];
   }
   c.flip ^= 1;  // the next call writes the other copy, so no peer still reads this one
-  if (before) *before = pre;
-  return all;
 }
-
-// Exclusive sum of v over the block's threads before this one.
-HXM_DEV u64 block_before(Ctx& c, u64 v) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  u64 a = v;
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 x = __shfl_up_sync(0xffffffffu, a, o);
-    if (lane >= o) a += x;
-  }
+// The block's sum of v, to all of its threads.
+HXM_DEV u64 block_sum(Shared* s, u64 v) {
+  v = warp_sum(v);
   __syncthreads();
-  if (lane == 31) c.s->scan[1][warp] = a;
+  if ((threadIdx.x & 31) == 0) s->scan[threadIdx.x >> 5] = v;
   __syncthreads();
-  u64 pre = a - v;
-  for (int i = 0; i < warp; ++i) pre += c.s->scan[1][i];
-  return pre;
+  return warp_sum(s->scan[threadIdx.x & 31]);
 }
 
 // The key at which the sum of f over larger keys first reaches past `target`: largest key K with
 // sum(f, key > K) <= target < sum(f, key >= K); `above` = sum(f, key > K).  The total exceeds target.
-template <typename F>
-HXM_DEV uint32_t select(Ctx& c, u64 target, u64* above, F f) {
+template <typename T, typename F>
+HXM_DEV uint32_t select(Ctx<T>& c, u64 target, u64* above, F f) {
+  Radix* rx = reinterpret_cast<Radix*>(c.region);
   uint32_t prefix = 0;
   u64 over = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    u64* hist = c.s->hist[(shift >> 3) & 1];
+  c.cl.sync();  // the region's last readers are done
+  for (int shift = Key<T>::kBits - 8; shift >= 0; shift -= 8) {
+    u64* hist = rx->hist[(shift >> 3) & 1];
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += kThreads) hist[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < c.n; i += kThreads) {
       const uint32_t k = c.keys[i];
-      if (k && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))) {
-        const u64 v = f(k, i);
+      if (k && (shift == Key<T>::kBits - 8 || (k >> (shift + 8)) == (prefix >> (shift + 8)))) {
+        const u64 v = f(k);
         if (v) atomicAdd(&hist[(k >> shift) & 255], v);
       }
     }
@@ -140,23 +232,19 @@ HXM_DEV uint32_t select(Ctx& c, u64 target, u64* above, F f) {
     for (int i = threadIdx.x; i < 256; i += kThreads) {
       u64 a = 0;
       for (unsigned r = 0; r < c.cl.num_blocks(); ++r) a += c.cl.map_shared_rank(hist, r)[i];
-      c.s->total[i] = a;
+      rx->total[i] = a;
     }
     __syncthreads();
     if (threadIdx.x < 32) {  // from the top: 8 bins a lane
       const int lane = threadIdx.x;
       u64 mine = 0;
-      for (int j = 0; j < 8; ++j) mine += c.s->total[255 - (lane * 8 + j)];
-      u64 a = mine;
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, a, o);
-        if (lane >= o) a += x;
-      }
+      for (int j = 0; j < 8; ++j) mine += rx->total[255 - (lane * 8 + j)];
+      const u64 a = warp_prefix(mine);
       u64 run = over + a - mine;
       if (run <= target && target < over + a) {
         for (int j = 0; j < 8; ++j) {
           const int bin = 255 - (lane * 8 + j);
-          const u64 v = c.s->total[bin];
+          const u64 v = rx->total[bin];
           if (target < run + v) {
             c.s->pick = bin;
             c.s->above = run;
@@ -170,146 +258,503 @@ HXM_DEV uint32_t select(Ctx& c, u64 target, u64* above, F f) {
     prefix |= (uint32_t)c.s->pick << shift;
     over = c.s->above;
   }
+  c.cl.sync();
   *above = over;
   return prefix;
 }
 
+// Puts the tokens whose key passes `want` into rank 0's list, as (key, ~token): larger is better.
+// The list's order is arbitrary; it is ranked next.
+template <typename T, typename F>
+HXM_DEV void gather(Ctx<T>& c, int i0, F want) {
+  Lists* ls = reinterpret_cast<Lists*>(c.cl.map_shared_rank(c.region, 0));
+  uint32_t* count = c.cl.map_shared_rank(&c.s->n_list, 0);
+  for (int i = threadIdx.x; i < c.n; i += kThreads) {
+    const uint32_t k = c.keys[i];
+    if (k && want(k)) {
+      const uint32_t at = atomicAdd(count, 1u);
+      if (at < kList) ls->item[at] = ((u64)k << 32) | (0xffffffffu - (uint32_t)(i0 + i));
+    }
+  }
+}
+// This thread's item of n <= kList listed ones, in rank order (0 past the end); rank 0's CTA only.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
-  extern __shared__ __align__(16) uint32_t keys[];
+HXM_DEV u64 ranked(Ctx<T>& c, int n) {
+  Lists* ls = reinterpret_cast<Lists*>(c.region);
+  u64 mine = 0;
+  int rank = 0;
+  if ((int)threadIdx.x < n) {
+    mine = ls->item[threadIdx.x];
+    for (int j = 0; j < n; ++j) rank += ls->item[j] > mine;
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < n) ls->item[rank] = mine;
+  __syncthreads();
+  return (int)threadIdx.x < n ? ls->item[threadIdx.x] : 0;
+}
+
+// From counts of 4096 bins (this thread: 4 tid ..), w_hi(b) >= every weight of bin b >= w_lo(b), the
+// weight `before` ahead of them and bounds of the border: tokens of bins below b0 lie before the border
+// for certain, those of bins behind b1 after it.
+template <typename FH, typename FL>
+HXM_DEV void border_bins(Shared* s, const uint32_t (&cnt)[4], float before, float border_lo, float border_hi, bool of_all,
+                         FH w_hi, FL w_lo, int& b0, int& b1) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float hi[4], lo[4], hs = 0.f, ls = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    hi[j] = cnt[j] * w_hi(4 * tid + j);
+    lo[j] = cnt[j] * w_lo(4 * tid + j);
+    hs += hi[j];
+    ls += lo[j];
+  }
+  float hp = hs, lp = ls;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float a = __shfl_up_sync(0xffffffffu, hp, o), b = __shfl_up_sync(0xffffffffu, lp, o);
+    if (lane >= o) {
+      hp += a;
+      lp += b;
+    }
+  }
+  __syncthreads();
+  if (lane == 31) {
+    s->wredf[0][warp] = hp;
+    s->wredf[1][warp] = lp;
+  }
+  if (tid == 0) s->pick = s->pick2 = kBins - 1;
+  __syncthreads();
+  float ha = 0.f, la = 0.f, hr = hp - hs, lr = lp - ls;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      hr += s->wredf[0][w];
+      lr += s->wredf[1][w];
+    }
+    ha += s->wredf[0][w];
+    la += s->wredf[1][w];
+  }
+  if (of_all) {  // the border is given as a share of the sum
+    border_lo *= la;
+    border_hi *= ha;
+  }
+  hr += before;
+  lr += before;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    hr += hi[j];
+    lr += lo[j];
+    if (hr >= border_lo && cnt[j]) atomicMin(&s->pick, 4 * tid + j);
+    if (lr > border_hi) atomicMin(&s->pick2, 4 * tid + j);
+  }
+  __syncthreads();
+  b0 = s->pick;
+  b1 = max(b0, s->pick2);
+  __syncthreads();
+}
+
+template <typename T>
+HXM_DEV float log_prob(const Ctx<T>& c, uint32_t key, u64 w, u64 total) {
+  if (w == total) return 0.f;
+  const double t = key == c.kmax ? 0.0 : ((double)Key<T>::value(key) - c.max) * c.c * 0.69314718055994530942;
+  return (float)(t - log((double)total * (1.0 / 17592186044416.0)));
+}
+
+// floor(u * total), held below total
+HXM_DEV u64 draw_target(float u, u64 total) {
+  const u64 t = (u64)floor(fmin(fmax((double)u, 0.0), 1.0) * (double)total);
+  return t < total ? t : total - 1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
+  typedef typename Key<T>::type K;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
   __shared__ Shared sh;
-  Ctx c{cg::this_cluster(), &sh, keys, 0, 0, 0, 1, 0, 0};
+  unsigned char* region = raw_smem;
+  K* keys = reinterpret_cast<K*>(raw_smem + kRegion);
+  Ctx<T> c{cg::this_cluster(), &sh, region, keys, 0, 0, 0, 0.f, 0.f, 0, 0};
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / c.cl.num_blocks(), rank = c.cl.block_rank();
   const int i0 = rank * p.slice;
   c.n = max(0, min(p.slice, p.vocab - i0));
-  c.e = ((c.n + kThreads - 1) / kThreads) | 1;
+  if (tid < 64) sh.pow2[tid] = exp2(tid / 64.0);
+  if (tid == 0) sh.n_list = 0;
+  for (int i = tid; i < kBins; i += kThreads) reinterpret_cast<Bins*>(region)->n[i] = 0;
+
+  // ---- logits -> keys, and the largest ----
   const T* lg = static_cast<const T*>(p.logits) + row * p.row_stride + i0;
-  // logits -> keys, and the largest
   uint32_t m = 0;
   constexpr int V = 16 / sizeof(T);
+  int done = 0;
   if (reinterpret_cast<uintptr_t>(lg) % 16 == 0) {
     const int nv = c.n / V;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < nv; i += kThreads) {
+    for (int i = tid; i < nv; i += kThreads) {
       const uint4 raw = __ldg(reinterpret_cast<const uint4*>(lg) + i);
       const T* x = reinterpret_cast<const T*>(&raw);
+      uint4 packed;
+      K* k = reinterpret_cast<K*>(&packed);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const uint32_t k = key_of(to_f32<T>(x[j]));
-        keys[i * V + j] = k;
-        m = max(m, k);
+        const uint32_t key = Key<T>::make(x[j]);
+        k[j] = (K)key;
+        m = max(m, key);
       }
+      reinterpret_cast<uint4*>(keys)[i] = packed;
     }
-    for (int i = nv * V + threadIdx.x; i < c.n; i += kThreads) {
-      const uint32_t k = key_of(to_f32<T>(lg[i]));
-      keys[i] = k;
-      m = max(m, k);
-    }
-  } else {
-    for (int i = threadIdx.x; i < c.n; i += kThreads) {
-      const uint32_t k = key_of(to_f32<T>(lg[i]));
-      keys[i] = k;
-      m = max(m, k);
-    }
+    done = nv * V;
+  }
+  for (int i = done + tid; i < c.n; i += kThreads) {
+    const uint32_t key = Key<T>::make(lg[i]);
+    keys[i] = (K)key;
+    m = max(m, key);
   }
   m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0) sh.wmax[threadIdx.x >> 5] = m;
+  if (lane == 0) sh.wred[warp] = m;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kWarps; ++i) m = max(m, sh.wmax[i]);
-    sh.cmax = m;
-  }
+  m = __reduce_max_sync(0xffffffffu, sh.wred[lane]);
+  if (tid == 0) sh.cmax = m;
   c.cl.sync();
   for (unsigned r = 0; r < c.cl.num_blocks(); ++r) c.kmax = max(c.kmax, *c.cl.map_shared_rank(&sh.cmax, r));
+
+  const float temp = p.temperature_rows ? p.temperature_rows[row] : p.temperature;
+  int k = p.top_k_rows ? p.top_k_rows[row] : p.top_k;
+  const float top_p = p.top_p_rows ? p.top_p_rows[row] : p.top_p;
+  const float min_p = p.min_p_rows ? p.min_p_rows[row] : p.min_p;
   if (c.kmax == 0) {  // nothing left (every CTA of the cluster agrees)
-    if (rank == 0 && threadIdx.x == 0) {
+    if (rank == 0 && tid == 0) {
       p.tokens[row] = -1;
       if (p.logprob) p.logprob[row] = -INFINITY;
     }
     c.cl.sync();
     return;
   }
-  const float temp = p.temperature_rows ? p.temperature_rows[row] : p.temperature;
-  const bool greedy = !(temp > 0.f);
-  int k = p.top_k_rows ? p.top_k_rows[row] : p.top_k;
-  if (greedy) k = 1;
-  const float top_p = greedy ? 1.f : p.top_p_rows ? p.top_p_rows[row] : p.top_p;
-  const float min_p = greedy ? 0.f : p.min_p_rows ? p.min_p_rows[row] : p.min_p;
-  c.max = (double)logit_of(c.kmax);
-  c.t = greedy ? 1.0 : (double)temp;
+  if (!(temp > 0.f) || k == 1) {  // the lowest token with the largest logit
+    uint32_t at = 0xffffffffu;
+    for (int i = tid; i < c.n; i += kThreads)
+      if (keys[i] == c.kmax) {
+        at = i0 + i;
+        break;
+      }
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (lane == 0) sh.wred[warp] = at;
+    __syncthreads();
+    if (warp == 0) {
+      at = __reduce_min_sync(0xffffffffu, sh.wred[lane]);
+      if (lane == 0) sh.cmin[0] = at;
+    }
+    c.cl.sync();
+    if (rank == 0 && tid == 0) {
+      for (unsigned r = 1; r < c.cl.num_blocks(); ++r) at = min(at, *c.cl.map_shared_rank(&sh.cmin[0], r));
+      p.tokens[row] = at;
+      if (p.logprob) p.logprob[row] = 0.f;
+    }
+    c.cl.sync();
+    return;
+  }
+  c.fmax = Key<T>::value(c.kmax);
+  c.max = (double)c.fmax;
+  c.c = 1.4426950408889634074 / (double)temp;
+  c.per_bin = kBinsPerUnit / temp;
+  const double min_w = (double)min_p * 17592186044416.0;
+  const float u = p.uniforms[row];
 
   // kept: key > thr, and the first `ties` tokens whose key is thr
   uint32_t thr = 0;
   u64 ties = 0;
-  if (k == 1) {
-    thr = c.kmax;
-    ties = 1;
-  } else if (k > 0 && k < p.vocab) {
-    u64 valid = 0;
-    for (int i = threadIdx.x; i < c.n; i += kThreads) valid += keys[i] != 0;
-    if (cluster_sum(c, valid, nullptr) > (u64)k) {
+  bool all_ties = true;  // no token of key thr is dropped
+  if ((k > 0 && k < p.vocab) || top_p < 1.f) {
+    // ---- counts per bin, over the cluster; this thread: bins 4 tid .. ----
+    Bins* bins = reinterpret_cast<Bins*>(region);
+    for (int i = tid; i < c.n; i += kThreads) {
+      const uint32_t key = keys[i];
+      if (key) atomicAdd(&bins->n[bin_of(c, key)], 1u);
+    }
+    c.cl.sync();
+    uint32_t cnt[4] = {0, 0, 0, 0};
+    for (unsigned r = 0; r < c.cl.num_blocks(); ++r) {
+      const uint4 x = reinterpret_cast<const uint4*>(c.cl.map_shared_rank(bins, r))[tid];
+      cnt[0] += x.x;
+      cnt[1] += x.y;
+      cnt[2] += x.z;
+      cnt[3] += x.w;
+    }
+    const uint32_t four = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    const uint32_t upto = (uint32_t)block_prefix(&sh, four), from = upto - four;
+    __syncthreads();
+    if (tid == kThreads - 1) sh.pick = (int)upto;
+    __syncthreads();
+    const int valid = sh.pick;
+    if (k >= valid) k = 0;
+    c.cl.sync();  // every CTA has read the bins: the region is free
+    if (k > 0) {
+      uint32_t run = from;
+      for (int j = 0; j < 4; ++j) {
+        if (run < (uint32_t)k && (uint32_t)k <= run + cnt[j]) {
+          sh.pick = 4 * tid + j;
+          sh.pick2 = (int)(run + cnt[j]);
+        }
+        run += cnt[j];
+      }
+      __syncthreads();
+      const int last = sh.pick, listed = sh.pick2;
+      if (k <= kTopKList && listed <= kList) {
+        // ---- the k largest as a list in rank 0: rank, cut, draw ----
+        gather(c, i0, [&](uint32_t key) { return bin_of(c, key) <= last; });
+        c.cl.sync();
+        if (rank != 0) return;
+        Lists* ls = reinterpret_cast<Lists*>(region);
+        const u64 item = ranked(c, listed);
+        const uint32_t key = (uint32_t)(item >> 32);
+        const double wd = tid < k ? weight_d(c, key) : 0.0;
+        const u64 w = to_fixed(wd);
+        const u64 incl = block_prefix(&sh, w);
+        ls->weight[tid] = incl;
+        __syncthreads();
+        const u64 all = ls->weight[kThreads - 1];
+        const u64 border = top_p < 1.f ? (u64)floor(fmax((double)top_p, 0.0) * (double)all) : all;
+        // a first run of the ranking: both cuts fall with the weight
+        const bool keep = tid < k && (tid == 0 || incl - w <= border) && (wd >= min_w || key == c.kmax);
+        const int kept = __syncthreads_count(keep);
+        const u64 total = ls->weight[kept - 1];
+        const u64 target = draw_target(u, total);
+        __syncthreads();
+        ls->weight[tid] = keep ? w : 0;
+        __syncthreads();
+        if (tid < kept) {  // the weights of the kept tokens up to this one, in the order of the tokens
+          u64 sum = 0;
+          const uint32_t me = (uint32_t)item;  // ~token: larger for lower tokens
+          for (int j = 0; j < kept; ++j) sum += (uint32_t)ls->item[j] >= me ? ls->weight[j] : 0;
+          if (target < sum && sum - w <= target) {
+            p.tokens[row] = (int64_t)(0xffffffffu - me);
+            if (p.logprob) p.logprob[row] = log_prob(c, key, w, total);
+          }
+        }
+        return;
+      }
       u64 above;
-      thr = select(c, (u64)(k - 1), &above, [](uint32_t, int) { return (u64)1; });
+      thr = select(c, (u64)(k - 1), &above, [](uint32_t) { return (u64)1; });
       ties = (u64)k - above;
+      all_ties = false;
+    }
+    if (top_p < 1.f) {
+      bool settled = false;
+      if (k == 0) {
+        // ---- the bins that may hold the border, from the counts; all weights, and those before ----
+        int b0, b1;
+        const float share = fmaxf(top_p, 0.f);
+        border_bins(&sh, cnt, 0.f, share, share, true,
+                    [](int b) { return expf(-(float)b / kBinsPerUnit) * 1.001f; },
+                    [](int b) { return b == kBins - 1 ? 0.f : expf(-(float)(b + 1) / kBinsPerUnit) * 0.999f; }, b0, b1);
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) in += 4 * tid + j >= b0 && 4 * tid + j <= b1 ? cnt[j] : 0;
+        int listed = (int)block_sum(&sh, in);
+        u64 sum = 0, before = 0;
+        for (int i = tid; i < c.n; i += kThreads) {
+          const uint32_t key = keys[i];
+          if (key) {
+            const u64 w = weight(c, key);
+            sum += w;
+            if (bin_of(c, key) < b0) before += w;
+          }
+        }
+        sum = block_sum(&sh, sum);
+        before = block_sum(&sh, before);
+        u64 all, pre, unused;
+        cluster_sum(c, sum, before, all, pre, unused);
+        const u64 border = (u64)floor(fmax((double)top_p, 0.0) * (double)all);
+        // finer bins over b0 .. b1
+        const float from = b0 / c.per_bin, per_fine = c.per_bin * (float)kBins / (float)(b1 - b0 + 1);
+        auto fine_of = [&](uint32_t key) {
+          const float f = ((c.fmax - Key<T>::value(key)) - from) * per_fine;
+          return key == c.kmax || !(f > 0.f) ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
+        };
+        auto inside = [&](uint32_t key) {
+          const int b = bin_of(c, key);
+          return b >= b0 && b <= b1;
+        };
+        int f0 = 0, f1 = kBins - 1;
+        if (listed > kList) {
+          Bins* bins = reinterpret_cast<Bins*>(region);
+          for (int i = tid; i < kBins; i += kThreads) bins->n[i] = 0;
+          __syncthreads();
+          for (int i = tid; i < c.n; i += kThreads) {
+            const uint32_t key = keys[i];
+            if (key && inside(key)) atomicAdd(&bins->n[fine_of(key)], 1u);
+          }
+          c.cl.sync();
+          uint32_t fine[4] = {0, 0, 0, 0};
+          for (unsigned r = 0; r < c.cl.num_blocks(); ++r) {
+            const uint4 x = reinterpret_cast<const uint4*>(c.cl.map_shared_rank(bins, r))[tid];
+            fine[0] += x.x;
+            fine[1] += x.y;
+            fine[2] += x.z;
+            fine[3] += x.w;
+          }
+          c.cl.sync();
+          const float unit = 1.f / 17592186044416.f, step = 1.f / (per_fine * temp), start = from / temp;
+          const float b = (float)border * unit;
+          border_bins(&sh, fine, (float)pre * unit, b * 0.999999f, b * 1.000001f, false,
+                      [&](int j) { return expf(-(start + j * step)) * 1.001f; },
+                      [&](int j) { return expf(-(start + (j + 1) * step)) * 0.999f; }, f0, f1);
+          in = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) in += 4 * tid + j >= f0 && 4 * tid + j <= f1 ? fine[j] : 0;
+          listed = (int)block_sum(&sh, in);
+          before = 0;  // those inside that come before the finer bins
+          for (int i = tid; i < c.n; i += kThreads) {
+            const uint32_t key = keys[i];
+            if (key && inside(key) && fine_of(key) < f0) before += weight(c, key);
+          }
+          before = block_sum(&sh, before);
+          u64 more, unused2;
+          cluster_sum(c, before, 0, more, unused, unused2);
+          pre += more;
+        }
+        if (listed <= kList) {
+          gather(c, i0, [&](uint32_t key) {
+            if (!inside(key)) return false;
+            const int f = fine_of(key);
+            return f >= f0 && f <= f1;
+          });
+          c.cl.sync();
+          if (rank == 0) {
+            const u64 item = ranked(c, listed);
+            const uint32_t key = (uint32_t)(item >> 32);
+            const u64 w = tid < listed ? weight(c, key) : 0;
+            const u64 excl = pre + block_prefix(&sh, w) - w;
+            const int kept = __syncthreads_count(tid < listed && excl <= border);
+            Lists* ls = reinterpret_cast<Lists*>(region);
+            const uint32_t t = (uint32_t)(ls->item[max(kept - 1, 0)] >> 32);
+            const int eq = __syncthreads_count(tid < kept && key == t), eq_all = __syncthreads_count(tid < listed && key == t);
+            if (tid == 0) {
+              sh.thr = t;
+              sh.ties = eq;
+              sh.pick = eq == eq_all;
+            }
+          }
+          c.cl.sync();
+          thr = *c.cl.map_shared_rank(&sh.thr, 0);
+          ties = *c.cl.map_shared_rank(&sh.ties, 0);
+          all_ties = *c.cl.map_shared_rank(&sh.pick, 0) != 0;
+          c.cl.sync();
+          settled = true;
+        }
+      }
+      if (!settled) {
+        // ---- weights by radix; the tokens tied at the top-k border count `ties` times, once ----
+        auto kept_weight = [&](uint32_t key) { return key > thr ? weight(c, key) : (u64)0; };
+        u64 sum = 0;
+        for (int i = tid; i < c.n; i += kThreads) sum += keys[i] ? kept_weight(keys[i]) : (u64)0;
+        sum = block_sum(&sh, sum);
+        u64 larger, unused, unused2;
+        cluster_sum(c, sum, 0, larger, unused, unused2);
+        const u64 wt = thr ? weight(c, thr) : 0;
+        const u64 total = larger + ties * wt;
+        const u64 target = (u64)floor(fmax((double)top_p, 0.0) * (double)total);
+        if (target < total) {
+          if (larger > target) {
+            u64 above;
+            const uint32_t t2 = select(c, target, &above, kept_weight);
+            ties = (target - above) / weight(c, t2) + 1;
+            thr = t2;
+          } else {
+            const u64 stay = wt ? (target - larger) / wt + 1 : ties;
+            ties = min(ties, stay);
+          }
+          all_ties = false;
+        }
+      }
     }
   }
-  auto kept_weight = [&](uint32_t key) { return key > thr ? weight(c, key) : (u64)0; };
-  if (top_p < 1.f && k != 1) {
+
+  // ---- the draw, in the order of the tokens: sums of kSubs runs, four per warp ----
+  const int run = ((c.n + kSubs - 1) / kSubs + 31) / 32 * 32;
+  u64 tie_pre[4] = {0, 0, 0, 0};  // tied tokens before each of this warp's runs
+  if (!all_ties) {
     u64 mine = 0;
-    for (int i = threadIdx.x; i < c.n; i += kThreads) mine += keys[i] ? kept_weight(keys[i]) : (u64)0;
-    const u64 wt = thr ? weight(c, thr) : 0;
-    const u64 total = cluster_sum(c, mine, nullptr) + ties * wt;
-    const double border = fmax((double)top_p, 0.0) * (double)total;  // a token stays with at most this before it
-    const u64 target = (u64)floor(border);
-    if (target < total) {
-      u64 above;
-      // the tied tokens at the top-k border count `ties` times, once for the cluster
-      u64 in_larger = total - ties * wt;
-      if (in_larger > target) {
-        const uint32_t t2 = select(c, target, &above, [&](uint32_t key, int) { return kept_weight(key); });
-        ties = (target - above) / weight(c, t2) + 1;
-        thr = t2;
-      } else {
-        const u64 stay = wt ? (target - in_larger) / wt + 1 : ties;
-        ties = min(ties, stay);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t t = 0;
+      const int lo = (4 * warp + q) * run, hi = min(c.n, lo + run);
+      for (int i = lo + lane; i < hi; i += 32) t += keys[i] == thr;
+      tie_pre[q] = mine;
+      mine += __reduce_add_sync(0xffffffffu, t);
+    }
+    const u64 incl = block_prefix(&sh, lane == 0 ? mine : 0);  // up to this warp's end
+    if (tid == kThreads - 1) sh.above = incl;
+    __syncthreads();
+    u64 all, unused, before;
+    cluster_sum(c, sh.above, 0, all, unused, before);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) tie_pre[q] += before + incl - mine;
+  }
+  // weight of token i (within the warp's step of 32 tokens) given the tied tokens before the step
+  auto drawn = [&](int i, int hi, u64& tied) -> u64 {
+    const uint32_t key = i < hi ? keys[i] : 0;
+    bool keep = key > thr;
+    if (thr) {
+      const bool tie = key == thr;
+      const uint32_t same = __ballot_sync(0xffffffffu, tie);
+      if (tie) keep = all_ties || tied + __popc(same & ((1u << lane) - 1)) < ties;
+      tied += __popc(same);
+    }
+    if (!keep) return 0;
+    const double w = weight_d(c, key);
+    return w >= min_w || key == c.kmax ? to_fixed(w) : 0;
+  };
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int lo = (4 * warp + q) * run, hi = min(c.n, lo + run);
+    u64 sum = 0, tied = tie_pre[q];
+    for (int i = lo; i < hi; i += 32) sum += drawn(i + lane, hi, tied);
+    sum = warp_sum(sum);
+    if (lane == 0) sh.sub[4 * warp + q] = sum;
+  }
+  if (tid == 0) sh.run_at = -1;
+  __syncthreads();
+  u64 part[4] = {0, 0, 0, 0}, mine = 0, upto = 0;
+  if (warp == 0) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      part[q] = sh.sub[4 * lane + q];
+      mine += part[q];
+    }
+    upto = warp_prefix(mine);
+    if (lane == 31) sh.above = upto;
+  }
+  __syncthreads();
+  u64 total, unused, before;
+  cluster_sum(c, sh.above, 0, total, unused, before);
+  const u64 target = draw_target(u, total);
+  if (warp == 0) {  // the run that holds the target
+    u64 at = before + upto - mine;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (at <= target && target < at + part[q]) {
+        sh.run_at = 4 * lane + q;
+        sh.run_sum = at;
       }
+      at += part[q];
     }
   }
-  // drop by min-p, then the draw: runs of c.e tokens per thread, in the order of the tokens
-  const int lo = min(c.n, (int)threadIdx.x * c.e), hi = min(c.n, lo + c.e);
-  u64 tied = 0;
-  for (int i = lo; i < hi; ++i) tied += thr && keys[i] == thr;
-  u64 tie_pre = 0;
-  cluster_sum(c, tied, &tie_pre);
-  tie_pre += block_before(c, tied);
-  auto draw_weight = [&](uint32_t key, u64& rank_of_tie) -> u64 {
-    if (key == 0 || key < thr) return 0;
-    if (key == thr && rank_of_tie++ >= ties) return 0;
-    const double w = weight_d(c, key);
-    return w >= (double)min_p || key == c.kmax ? (u64)__double2ll_rn(w * kOne) : 0;
-  };
-  u64 mine = 0, rk = tie_pre;
-  for (int i = lo; i < hi; ++i) mine += draw_weight(keys[i], rk);
-  u64 before = 0;
-  const u64 total = cluster_sum(c, mine, &before);
-  before += block_before(c, mine);
-  const double u = fmin(fmax((double)p.uniforms[row], 0.0), 1.0);
-  u64 target = (u64)floor(u * (double)total);
-  if (target >= total) target = total - 1;
-  if (before <= target && target < before + mine) {
-    rk = tie_pre;
-    u64 run = before;
-    for (int i = lo; i < hi; ++i) {
-      const u64 w = draw_weight(keys[i], rk);
-      run += w;
-      if (target < run) {
-        p.tokens[row] = i0 + i;
-        if (p.logprob) p.logprob[row] = keys[i] == c.kmax && w == total
-                                            ? 0.f
-                                            : (float)(((double)logit_of(keys[i]) == c.max ? 0.0 : ((double)logit_of(keys[i]) - c.max) / c.t) -
-                                                      log((double)total * (1.0 / kOne)));
-        break;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (sh.run_at != 4 * warp + q) continue;
+    const int lo = (4 * warp + q) * run, hi = min(c.n, lo + run);
+    u64 sum = sh.run_sum, tied = tie_pre[q];
+    for (int i = lo; i < hi; i += 32) {
+      const u64 w = drawn(i + lane, hi, tied);
+      const u64 incl = sum + warp_prefix(w);
+      if (target < incl && incl - w <= target) {
+        p.tokens[row] = i0 + i + lane;
+        if (p.logprob) p.logprob[row] = log_prob(c, (uint32_t)keys[i + lane], w, total);
       }
+      sum = __shfl_sync(0xffffffffu, incl, 31);
+      if (target < sum) break;
     }
   }
   c.cl.sync();  // a peer may still read this CTA's shared memory
@@ -317,12 +762,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
 
 template <typename T>
 static hxm_status launch(Params p, int rows, cudaStream_t st) {
-  // CTAs per row: as many as keep the slices within shared memory, more while the SMs are not full
+  typedef typename Key<T>::type K;
+  // CTAs per row: as many as keep the keys within shared memory, more while the SMs are not full
+  // (a row then goes through fewer tokens per thread)
+  const int most = (int)(200 * 1024 / sizeof(K));
   int cl = 1;
-  while ((p.vocab + cl - 1) / cl > 50 * 1024) cl *= 2;
-  while (cl < 8 && (int64_t)rows * cl < 148 && p.vocab / cl > 4 * kThreads) cl *= 2;
+  while ((p.vocab + cl - 1) / cl > most) cl *= 2;
+  while (cl < 8 && (int64_t)rows * cl * 2 <= 148 && p.vocab / cl > 4 * kThreads) cl *= 2;
   p.slice = ((p.vocab + cl - 1) / cl + 7) / 8 * 8;
-  const size_t smem = (size_t)p.slice * sizeof(uint32_t);
+  const size_t smem = kRegion + (size_t)p.slice * sizeof(K);
   HXM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cl));
