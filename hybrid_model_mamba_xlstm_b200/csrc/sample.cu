@@ -6,14 +6,14 @@
 // cluster takes a row: the logits are read from HBM once and stay in shared memory as order-preserving
 // keys (16 bits for 16-bit logits).  What is left is a chain of passes over shared memory, and the
 // number of passes and of 64-bit exponentials in them is the cost:
-//   - counts of the logits in 4096 bins, 1/128 of exp's unit wide, below the largest one;
-//   - top_k up to 512: the tokens of the bins that hold the k largest (a few more than k) go to a list,
+//   - counts of the logits in 2048 bins, 1/64 of exp's unit wide, below the largest one;
+//   - top_k up to 400: the tokens of the bins that hold the k largest (a few more than k) go to a list,
 //     which alone is ranked, cut and drawn from;
-//   - top_p: bin counts bound the weight above every bin from both sides to 1 part in 100, so the
-//     border lies in a few bins; one pass sums all weights and those before these bins.  The tokens of
-//     the bins are listed and ranked, after counting them once more in 4096 finer bins where they are
-//     more than 1024;
-//   - anything else (a border among more than 1024 tokens): radix selection, 8 bits of the key a pass.
+//   - a larger top_k: the border's bin is known from the counts, and its keys are listed;
+//   - top_p: counts and mean places in the bins bound the weight above every bin to 1 part in 10^4, so the
+//     border lies in a bin or a few; the pass that sums all weights also sums those before them and lists their keys;
+//   - a list of keys is searched for the border by radix, 8 bits of the key a pass; so are all keys where
+//     the list would not fit (a border among thousands of tokens: logits of few values).
 //
 // Weights w = exp((logit - max) / temperature) are formed in 64 bits and held as integers of 2^-44:
 // their sums are exact, so no order of additions (atomics, cluster size) changes a result, and a
@@ -29,13 +29,13 @@ namespace cg = cooperative_groups;
 namespace hxm {
 namespace sample {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;  // two CTAs of 64 registers a thread fit an SM: one's barriers hide behind the other
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxVocab = 1 << 18;
-constexpr int kBins = 4096;
-constexpr float kBinsPerUnit = 128.f;  // 32 units in all: weights behind them are below 2^-46
-constexpr int kList = 1024;      // tokens ranked one by one
-constexpr int kTopKList = 512;   // top_k up to which the kept tokens are listed
+constexpr int kBins = 4 * kThreads;
+constexpr float kBinsPerUnit = 64.f;   // 32 units in all: weights behind them are below 2^-46
+constexpr int kList = kThreads;  // tokens ranked one by one
+constexpr int kTopKList = 400;   // top_k up to which the kept tokens are listed
 constexpr int kSubs = 4 * kWarps;  // runs of tokens whose weights are summed apart
 typedef unsigned long long u64;
 
@@ -89,10 +89,11 @@ template <> struct Key<__half> : Key16<__half> {};
 
 struct Shared {
   double pow2[64];  // 2^(j / 64)
-  u64 scan[kWarps];
+  u64 scan[32];     // by warp; the rest stay 0
   u64 mine[2][2];   // this CTA's totals, double-buffered, for the cluster to read
   u64 sub[kSubs];
-  uint32_t wred[kWarps];
+  u64 hist[256];    // select_listed
+  uint32_t wred[32];
   float wredf[2][kWarps];
   uint32_t cmax;
   uint32_t cmin[1];
@@ -106,10 +107,13 @@ struct Shared {
   u64 ties;
 };
 // One region after the keys: the bins, then a list and its ranking, or the radix selection's sums.
-struct Bins { uint32_t n[kBins]; };
+struct Bins { uint32_t n[kBins], pos[kBins]; };  // tokens, and their summed positions in the bin in 1/1024
 struct Lists { u64 item[kList]; u64 weight[kList]; };
 struct Radix { u64 hist[2][256]; u64 total[256]; };
+// Keys listed at a border.
+template <typename K> struct Keys { static constexpr int kMax = (int)(sizeof(Bins) / sizeof(K)); K key[kMax]; };
 constexpr size_t kRegion = sizeof(Bins);
+static_assert(kThreads * 4 <= kRegion / 2 && kThreads * 8 <= kRegion / 2, "select_few");
 static_assert(sizeof(Lists) <= kRegion && sizeof(Radix) <= kRegion, "region");
 
 template <typename T>
@@ -150,11 +154,11 @@ HXM_DEV u64 weight(const Ctx<T>& c, uint32_t key) { return to_fixed(weight_d(c, 
 
 // Bins of falling logits: 0 next to the largest, the last one open.
 template <typename T>
-HXM_DEV int bin_of(const Ctx<T>& c, uint32_t key) {
-  if (key == c.kmax) return 0;
-  const float b = (c.fmax - Key<T>::value(key)) * c.per_bin;
-  return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+HXM_DEV float place_of(const Ctx<T>& c, uint32_t key) {
+  return key == c.kmax ? 0.f : fminf((c.fmax - Key<T>::value(key)) * c.per_bin, (float)(kBins - 1));
 }
+template <typename T>
+HXM_DEV int bin_of(const Ctx<T>& c, uint32_t key) { return (int)place_of(c, key); }
 
 HXM_DEV u64 warp_sum(u64 v) {
 #pragma unroll
@@ -208,6 +212,27 @@ HXM_DEV u64 block_sum(Shared* s, u64 v) {
   return warp_sum(s->scan[threadIdx.x & 31]);
 }
 
+// The bin of 256 sums, from the top, at which `over` + the sum passes target (s->pick), and the sum before (s->above).
+HXM_DEV void pick_bin(Shared* s, const u64* sums, u64 over, u64 target) {
+  if (threadIdx.x >= 32) return;
+  const int lane = threadIdx.x;  // 8 bins a lane
+  u64 mine = 0;
+  for (int j = 0; j < 8; ++j) mine += sums[255 - (lane * 8 + j)];
+  const u64 a = warp_prefix(mine);
+  u64 run = over + a - mine;
+  if (run <= target && target < over + a)
+    for (int j = 0; j < 8; ++j) {
+      const int bin = 255 - (lane * 8 + j);
+      const u64 v = sums[bin];
+      if (target < run + v) {
+        s->pick = bin;
+        s->above = run;
+        break;
+      }
+      run += v;
+    }
+}
+
 // The key at which the sum of f over larger keys first reaches past `target`: largest key K with
 // sum(f, key > K) <= target < sum(f, key >= K); `above` = sum(f, key > K).  The total exceeds target.
 template <typename T, typename F>
@@ -221,11 +246,21 @@ HXM_DEV uint32_t select(Ctx<T>& c, u64 target, u64* above, F f) {
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += kThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < c.n; i += kThreads) {
-      const uint32_t k = c.keys[i];
-      if (k && (shift == Key<T>::kBits - 8 || (k >> (shift + 8)) == (prefix >> (shift + 8)))) {
-        const u64 v = f(k);
-        if (v) atomicAdd(&hist[(k >> shift) & 255], v);
+    for (int i0 = threadIdx.x & ~31; i0 < c.n; i0 += kThreads) {
+      const int i = i0 + (threadIdx.x & 31);
+      const uint32_t k = i < c.n ? c.keys[i] : 0;
+      const bool in = k && (shift == Key<T>::kBits - 8 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
+      const uint32_t who = __ballot_sync(0xffffffffu, in);
+      if (who == 0) continue;
+      const u64 v = in ? f(k) : 0;
+      const uint32_t bin = (k >> shift) & 255;
+      // the warps of a row of few values share a bin: one addition for all of their tokens
+      const uint32_t b0 = __shfl_sync(0xffffffffu, bin, __ffs(who) - 1);
+      if (__all_sync(0xffffffffu, !in || bin == b0)) {
+        const u64 sum = warp_sum(v);
+        if ((threadIdx.x & 31) == 0) atomicAdd(&hist[b0], sum);
+      } else if (v) {
+        atomicAdd(&hist[bin], v);
       }
     }
     c.cl.sync();
@@ -235,25 +270,7 @@ HXM_DEV uint32_t select(Ctx<T>& c, u64 target, u64* above, F f) {
       rx->total[i] = a;
     }
     __syncthreads();
-    if (threadIdx.x < 32) {  // from the top: 8 bins a lane
-      const int lane = threadIdx.x;
-      u64 mine = 0;
-      for (int j = 0; j < 8; ++j) mine += rx->total[255 - (lane * 8 + j)];
-      const u64 a = warp_prefix(mine);
-      u64 run = over + a - mine;
-      if (run <= target && target < over + a) {
-        for (int j = 0; j < 8; ++j) {
-          const int bin = 255 - (lane * 8 + j);
-          const u64 v = rx->total[bin];
-          if (target < run + v) {
-            c.s->pick = bin;
-            c.s->above = run;
-            break;
-          }
-          run += v;
-        }
-      }
-    }
+    pick_bin(c.s, rx->total, over, target);
     __syncthreads();
     prefix |= (uint32_t)c.s->pick << shift;
     over = c.s->above;
@@ -261,6 +278,69 @@ HXM_DEV uint32_t select(Ctx<T>& c, u64 target, u64* above, F f) {
   c.cl.sync();
   *above = over;
   return prefix;
+}
+
+// Appends the key of every lane with `want` to rank 0's list (the whole warp calls; the order is arbitrary).
+template <typename T>
+HXM_DEV void append(Keys<typename Key<T>::type>* list, uint32_t* count, bool want, uint32_t key) {
+  const uint32_t who = __ballot_sync(0xffffffffu, want);
+  if (who == 0) return;
+  const int lane = threadIdx.x & 31, first = __ffs(who) - 1;
+  uint32_t at = 0;
+  if (lane == first) at = atomicAdd(count, (uint32_t)__popc(who));
+  at = __shfl_sync(0xffffffffu, at, first) + __popc(who & ((1u << lane) - 1));
+  if (want && at < Keys<typename Key<T>::type>::kMax) list->key[at] = (typename Key<T>::type)key;
+}
+
+// select() over a list of n keys, by rank 0's CTA alone; `over`: the sum before the list.
+template <typename T, typename F>
+HXM_DEV uint32_t select_listed(Ctx<T>& c, int n, u64 over, u64 target, u64* above, F f) {
+  const Keys<typename Key<T>::type>* list = reinterpret_cast<const Keys<typename Key<T>::type>*>(c.region);
+  uint32_t prefix = 0;
+  for (int shift = Key<T>::kBits - 8; shift >= 0; shift -= 8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256; i += kThreads) c.s->hist[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t k = list->key[i];
+      if (shift == Key<T>::kBits - 8 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&c.s->hist[(k >> shift) & 255], f(k));
+    }
+    __syncthreads();
+    pick_bin(c.s, c.s->hist, over, target);
+    __syncthreads();
+    prefix |= (uint32_t)c.s->pick << shift;
+    over = c.s->above;
+  }
+  *above = over;
+  return prefix;
+}
+
+// The same for n <= kThreads keys: every thread sums f over the keys above its own.
+template <typename T, typename F>
+HXM_DEV uint32_t select_few(Ctx<T>& c, int n, u64 over, u64 target, u64* above, F f) {
+  const Keys<typename Key<T>::type>* list = reinterpret_cast<const Keys<typename Key<T>::type>*>(c.region);
+  u64* w = reinterpret_cast<u64*>(c.region + kRegion / 2);
+  const int tid = threadIdx.x;
+  const uint32_t mine = tid < n ? list->key[tid] : 0;
+  const u64 v = tid < n ? f(mine) : 0;
+  w[tid] = v;
+  __syncthreads();
+  if ((tid & ~31) < n) {
+    u64 larger = over, same = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const uint32_t k = list->key[j];
+      larger += k > mine ? w[j] : 0;
+      same += k == mine ? w[j] : 0;
+    }
+    if (tid < n && larger <= target && target < larger + same) {  // all threads of this key agree
+      c.s->pick = (int)mine;
+      c.s->above = larger;
+    }
+  }
+  __syncthreads();
+  *above = c.s->above;
+  return (uint32_t)c.s->pick;
 }
 
 // Puts the tokens whose key passes `want` into rank 0's list, as (key, ~token): larger is better.
@@ -293,18 +373,21 @@ HXM_DEV u64 ranked(Ctx<T>& c, int n) {
   return (int)threadIdx.x < n ? ls->item[threadIdx.x] : 0;
 }
 
-// From counts of 4096 bins (this thread: 4 tid ..), w_hi(b) >= every weight of bin b >= w_lo(b), the
-// weight `before` ahead of them and bounds of the border: tokens of bins below b0 lie before the border
-// for certain, those of bins behind b1 after it.
-template <typename FH, typename FL>
-HXM_DEV void border_bins(Shared* s, const uint32_t (&cnt)[4], float before, float border_lo, float border_hi, bool of_all,
-                         FH w_hi, FL w_lo, int& b0, int& b1) {
+// From the counts and mean places in the bins (this thread: 4 tid ..): tokens of bins below b0 lie before
+// the border, a share of the whole weight, for certain, and those of bins behind b1 after it.  The
+// weights of n tokens of one bin, 1/64 wide, sum to n e^-(mean place) times at most 1 + (1/64)^2 / 8
+// (Jensen's inequality from below, the largest variance from above); with the places' rounding that is
+// 1 part in 10^4.  `split`: a bin of which only some tokens count: bounded by its ends.
+HXM_DEV void border_bins(Shared* s, const uint32_t (&cnt)[4], const uint32_t (&pos)[4], int split, float share, int& b0, int& b1) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float hi[4], lo[4], hs = 0.f, ls = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    hi[j] = cnt[j] * w_hi(4 * tid + j);
-    lo[j] = cnt[j] * w_lo(4 * tid + j);
+    const int b = 4 * tid + j;
+    const float n = (float)cnt[j], mean = cnt[j] ? (float)pos[j] * (1.f / 1024.f) / n : 0.f;
+    const bool open = b == kBins - 1, part = b == split;
+    hi[j] = n * expf(-((float)b + (part || open ? 0.f : mean)) / kBinsPerUnit) * 1.0001f;
+    lo[j] = open ? 0.f : n * expf(-((float)b + (part ? 1.f : mean + 1.f / 1024.f)) / kBinsPerUnit) * 0.9999f;
     hs += hi[j];
     ls += lo[j];
   }
@@ -333,18 +416,12 @@ HXM_DEV void border_bins(Shared* s, const uint32_t (&cnt)[4], float before, floa
     ha += s->wredf[0][w];
     la += s->wredf[1][w];
   }
-  if (of_all) {  // the border is given as a share of the sum
-    border_lo *= la;
-    border_hi *= ha;
-  }
-  hr += before;
-  lr += before;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     hr += hi[j];
     lr += lo[j];
-    if (hr >= border_lo && cnt[j]) atomicMin(&s->pick, 4 * tid + j);
-    if (lr > border_hi) atomicMin(&s->pick2, 4 * tid + j);
+    if (hr >= share * la && cnt[j]) atomicMin(&s->pick, 4 * tid + j);
+    if (lr > share * ha) atomicMin(&s->pick2, 4 * tid + j);
   }
   __syncthreads();
   b0 = s->pick;
@@ -366,7 +443,7 @@ HXM_DEV u64 draw_target(float u, u64 total) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   typedef typename Key<T>::type K;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   __shared__ Shared sh;
@@ -379,7 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
   c.n = max(0, min(p.slice, p.vocab - i0));
   if (tid < 64) sh.pow2[tid] = exp2(tid / 64.0);
   if (tid == 0) sh.n_list = 0;
-  for (int i = tid; i < kBins; i += kThreads) reinterpret_cast<Bins*>(region)->n[i] = 0;
+  if (tid < 32) sh.scan[tid] = sh.wred[tid] = 0;
+  for (int i = tid; i < 2 * kBins; i += kThreads) reinterpret_cast<Bins*>(region)->n[i] = 0;
 
   // ---- logits -> keys, and the largest ----
   const T* lg = static_cast<const T*>(p.logits) + row * p.row_stride + i0;
@@ -410,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
     m = max(m, key);
   }
   m = __reduce_max_sync(0xffffffffu, m);
+  __syncthreads();
   if (lane == 0) sh.wred[warp] = m;
   __syncthreads();
   m = __reduce_max_sync(0xffffffffu, sh.wred[lane]);
@@ -441,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
     if (lane == 0) sh.wred[warp] = at;
     __syncthreads();
     if (warp == 0) {
-      at = __reduce_min_sync(0xffffffffu, sh.wred[lane]);
+      at = __reduce_min_sync(0xffffffffu, lane < kWarps ? sh.wred[lane] : 0xffffffffu);
       if (lane == 0) sh.cmin[0] = at;
     }
     c.cl.sync();
@@ -467,18 +546,30 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
   if ((k > 0 && k < p.vocab) || top_p < 1.f) {
     // ---- counts per bin, over the cluster; this thread: bins 4 tid .. ----
     Bins* bins = reinterpret_cast<Bins*>(region);
+    const bool cut = top_p < 1.f;
+#pragma unroll 4
     for (int i = tid; i < c.n; i += kThreads) {
       const uint32_t key = keys[i];
-      if (key) atomicAdd(&bins->n[bin_of(c, key)], 1u);
+      if (key) {
+        const float at = place_of(c, key);
+        const int bin = (int)at;
+        atomicAdd(&bins->n[bin], 1u);
+        if (cut) atomicAdd(&bins->pos[bin], (uint32_t)((at - (float)bin) * 1024.f));
+      }
     }
     c.cl.sync();
-    uint32_t cnt[4] = {0, 0, 0, 0};
+    uint32_t cnt[4] = {0, 0, 0, 0}, pos[4] = {0, 0, 0, 0};
     for (unsigned r = 0; r < c.cl.num_blocks(); ++r) {
-      const uint4 x = reinterpret_cast<const uint4*>(c.cl.map_shared_rank(bins, r))[tid];
+      const Bins* peer = c.cl.map_shared_rank(bins, r);
+      const uint4 x = reinterpret_cast<const uint4*>(peer->n)[tid], y = reinterpret_cast<const uint4*>(peer->pos)[tid];
       cnt[0] += x.x;
       cnt[1] += x.y;
       cnt[2] += x.z;
       cnt[3] += x.w;
+      pos[0] += y.x;
+      pos[1] += y.y;
+      pos[2] += y.z;
+      pos[3] += y.w;
     }
     const uint32_t four = cnt[0] + cnt[1] + cnt[2] + cnt[3];
     const uint32_t upto = (uint32_t)block_prefix(&sh, four), from = upto - four;
@@ -488,6 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
     const int valid = sh.pick;
     if (k >= valid) k = 0;
     c.cl.sync();  // every CTA has read the bins: the region is free
+    Keys<K>* keys0 = reinterpret_cast<Keys<K>*>(c.cl.map_shared_rank(region, 0));
+    uint32_t* count0 = c.cl.map_shared_rank(&sh.n_list, 0);
+    int split = -1;
     if (k > 0) {
       uint32_t run = from;
       for (int j = 0; j < 4; ++j) {
@@ -533,106 +627,95 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
         }
         return;
       }
-      u64 above;
-      thr = select(c, (u64)(k - 1), &above, [](uint32_t) { return (u64)1; });
-      ties = (u64)k - above;
+      // ---- the border's bin: its keys listed, the k-th largest found among them ----
+      __syncthreads();
+      if (tid == last / 4) {
+        uint32_t r = from;
+        for (int j = 0; j < last % 4; ++j) r += cnt[j];
+        sh.pick = (int)r;  // tokens before the bin
+      }
+      __syncthreads();
+      const int ahead = sh.pick;
+      if (listed - ahead <= Keys<K>::kMax) {
+        for (int i = warp * 32; i < c.n; i += kThreads) {
+          const uint32_t key = i + lane < c.n ? keys[i + lane] : 0;
+          append<T>(keys0, count0, key && bin_of(c, key) == last, key);
+        }
+        c.cl.sync();
+        if (rank == 0) {
+          u64 above;
+          const int n = listed - ahead;
+          auto one = [](uint32_t) { return (u64)1; };
+          const uint32_t t = n <= kThreads ? select_few(c, n, (u64)ahead, (u64)(k - 1), &above, one)
+                                           : select_listed(c, n, (u64)ahead, (u64)(k - 1), &above, one);
+          if (tid == 0) {
+            sh.thr = t;
+            sh.ties = (u64)k - above;
+            sh.n_list = 0;
+          }
+        }
+        c.cl.sync();
+        thr = *c.cl.map_shared_rank(&sh.thr, 0);
+        ties = *c.cl.map_shared_rank(&sh.ties, 0);
+        c.cl.sync();
+      } else {
+        u64 above;
+        thr = select(c, (u64)(k - 1), &above, [](uint32_t) { return (u64)1; });
+        ties = (u64)k - above;
+      }
       all_ties = false;
+      split = last;
+      // from here on the counts are those of the kept tokens
+      uint32_t r = from;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t now = cnt[j];
+        cnt[j] = r >= (uint32_t)k ? 0 : min(now, (uint32_t)k - r);
+        r += now;
+      }
     }
     if (top_p < 1.f) {
-      bool settled = false;
-      if (k == 0) {
-        // ---- the bins that may hold the border, from the counts; all weights, and those before ----
-        int b0, b1;
-        const float share = fmaxf(top_p, 0.f);
-        border_bins(&sh, cnt, 0.f, share, share, true,
-                    [](int b) { return expf(-(float)b / kBinsPerUnit) * 1.001f; },
-                    [](int b) { return b == kBins - 1 ? 0.f : expf(-(float)(b + 1) / kBinsPerUnit) * 0.999f; }, b0, b1);
-        uint32_t in = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) in += 4 * tid + j >= b0 && 4 * tid + j <= b1 ? cnt[j] : 0;
-        int listed = (int)block_sum(&sh, in);
-        u64 sum = 0, before = 0;
-        for (int i = tid; i < c.n; i += kThreads) {
-          const uint32_t key = keys[i];
-          if (key) {
-            const u64 w = weight(c, key);
-            sum += w;
-            if (bin_of(c, key) < b0) before += w;
-          }
-        }
-        sum = block_sum(&sh, sum);
-        before = block_sum(&sh, before);
-        u64 all, pre, unused;
-        cluster_sum(c, sum, before, all, pre, unused);
-        const u64 border = (u64)floor(fmax((double)top_p, 0.0) * (double)all);
-        // finer bins over b0 .. b1
-        const float from = b0 / c.per_bin, per_fine = c.per_bin * (float)kBins / (float)(b1 - b0 + 1);
-        auto fine_of = [&](uint32_t key) {
-          const float f = ((c.fmax - Key<T>::value(key)) - from) * per_fine;
-          return key == c.kmax || !(f > 0.f) ? 0 : f < (float)(kBins - 1) ? (int)f : kBins - 1;
-        };
-        auto inside = [&](uint32_t key) {
-          const int b = bin_of(c, key);
-          return b >= b0 && b <= b1;
-        };
-        int f0 = 0, f1 = kBins - 1;
-        if (listed > kList) {
-          Bins* bins = reinterpret_cast<Bins*>(region);
-          for (int i = tid; i < kBins; i += kThreads) bins->n[i] = 0;
-          __syncthreads();
-          for (int i = tid; i < c.n; i += kThreads) {
-            const uint32_t key = keys[i];
-            if (key && inside(key)) atomicAdd(&bins->n[fine_of(key)], 1u);
-          }
-          c.cl.sync();
-          uint32_t fine[4] = {0, 0, 0, 0};
-          for (unsigned r = 0; r < c.cl.num_blocks(); ++r) {
-            const uint4 x = reinterpret_cast<const uint4*>(c.cl.map_shared_rank(bins, r))[tid];
-            fine[0] += x.x;
-            fine[1] += x.y;
-            fine[2] += x.z;
-            fine[3] += x.w;
-          }
-          c.cl.sync();
-          const float unit = 1.f / 17592186044416.f, step = 1.f / (per_fine * temp), start = from / temp;
-          const float b = (float)border * unit;
-          border_bins(&sh, fine, (float)pre * unit, b * 0.999999f, b * 1.000001f, false,
-                      [&](int j) { return expf(-(start + j * step)) * 1.001f; },
-                      [&](int j) { return expf(-(start + (j + 1) * step)) * 0.999f; }, f0, f1);
-          in = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) in += 4 * tid + j >= f0 && 4 * tid + j <= f1 ? fine[j] : 0;
-          listed = (int)block_sum(&sh, in);
-          before = 0;  // those inside that come before the finer bins
-          for (int i = tid; i < c.n; i += kThreads) {
-            const uint32_t key = keys[i];
-            if (key && inside(key) && fine_of(key) < f0) before += weight(c, key);
-          }
-          before = block_sum(&sh, before);
-          u64 more, unused2;
-          cluster_sum(c, before, 0, more, unused, unused2);
-          pre += more;
-        }
-        if (listed <= kList) {
-          gather(c, i0, [&](uint32_t key) {
-            if (!inside(key)) return false;
-            const int f = fine_of(key);
-            return f >= f0 && f <= f1;
-          });
-          c.cl.sync();
+      // ---- the bins that may hold the border; all weights, those before the bins, and the bins' keys ----
+      int b0, b1;
+      const float share = fmaxf(top_p, 0.f);
+      border_bins(&sh, cnt, pos, split, share, b0, b1);
+      u64 sum = 0, before = 0;
+#pragma unroll 2
+      for (int i = warp * 32; i < c.n; i += kThreads) {
+        const uint32_t key = i + lane < c.n ? keys[i + lane] : 0;
+        const bool in = key > thr;
+        const int bin = in ? bin_of(c, key) : kBins;
+        const u64 w = in ? weight(c, key) : 0;
+        sum += w;
+        if (bin < b0) before += w;
+        append<T>(keys0, count0, in && bin >= b0 && bin <= b1, key);
+      }
+      sum = block_sum(&sh, sum);
+      before = block_sum(&sh, before);
+      u64 larger, pre, unused;
+      cluster_sum(c, sum, before, larger, pre, unused);
+      // the tokens tied at the top-k border count `ties` times
+      const u64 wt = thr ? weight(c, thr) : 0;
+      const u64 total = larger + ties * wt;
+      const u64 target = (u64)floor(fmax((double)top_p, 0.0) * (double)total);  // a token stays with at most this before it
+      const int n = (int)*c.cl.map_shared_rank(count0, 0);
+      if (target < total) {
+        if (target >= larger) {
+          const u64 stay = wt ? (target - larger) / wt + 1 : ties;
+          ties = min(ties, stay);
+          all_ties = false;
+        } else if (n <= Keys<K>::kMax) {
           if (rank == 0) {
-            const u64 item = ranked(c, listed);
-            const uint32_t key = (uint32_t)(item >> 32);
-            const u64 w = tid < listed ? weight(c, key) : 0;
-            const u64 excl = pre + block_prefix(&sh, w) - w;
-            const int kept = __syncthreads_count(tid < listed && excl <= border);
-            Lists* ls = reinterpret_cast<Lists*>(region);
-            const uint32_t t = (uint32_t)(ls->item[max(kept - 1, 0)] >> 32);
-            const int eq = __syncthreads_count(tid < kept && key == t), eq_all = __syncthreads_count(tid < listed && key == t);
+            u64 above;
+            auto weighed = [&](uint32_t key) { return weight(c, key); };
+            const uint32_t t = n <= kThreads ? select_few(c, n, pre, target, &above, weighed) : select_listed(c, n, pre, target, &above, weighed);
+            uint32_t same = 0;
+            const Keys<K>* list = reinterpret_cast<const Keys<K>*>(region);
+            for (int i = tid; i < n; i += kThreads) same += list->key[i] == t;
+            const u64 all = block_sum(&sh, same), stay = (target - above) / weight(c, t) + 1;
             if (tid == 0) {
               sh.thr = t;
-              sh.ties = eq;
-              sh.pick = eq == eq_all;
+              sh.ties = min(all, stay);
+              sh.pick = all <= stay;
             }
           }
           c.cl.sync();
@@ -640,30 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
           ties = *c.cl.map_shared_rank(&sh.ties, 0);
           all_ties = *c.cl.map_shared_rank(&sh.pick, 0) != 0;
           c.cl.sync();
-          settled = true;
-        }
-      }
-      if (!settled) {
-        // ---- weights by radix; the tokens tied at the top-k border count `ties` times, once ----
-        auto kept_weight = [&](uint32_t key) { return key > thr ? weight(c, key) : (u64)0; };
-        u64 sum = 0;
-        for (int i = tid; i < c.n; i += kThreads) sum += keys[i] ? kept_weight(keys[i]) : (u64)0;
-        sum = block_sum(&sh, sum);
-        u64 larger, unused, unused2;
-        cluster_sum(c, sum, 0, larger, unused, unused2);
-        const u64 wt = thr ? weight(c, thr) : 0;
-        const u64 total = larger + ties * wt;
-        const u64 target = (u64)floor(fmax((double)top_p, 0.0) * (double)total);
-        if (target < total) {
-          if (larger > target) {
-            u64 above;
-            const uint32_t t2 = select(c, target, &above, kept_weight);
-            ties = (target - above) / weight(c, t2) + 1;
-            thr = t2;
-          } else {
-            const u64 stay = wt ? (target - larger) / wt + 1 : ties;
-            ties = min(ties, stay);
-          }
+        } else {
+          const uint32_t floor_key = thr;
+          u64 above;
+          thr = select(c, target, &above, [&](uint32_t key) { return key > floor_key ? weight(c, key) : (u64)0; });
+          ties = (target - above) / weight(c, thr) + 1;
           all_ties = false;
         }
       }
@@ -709,17 +773,19 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
   for (int q = 0; q < 4; ++q) {
     const int lo = (4 * warp + q) * run, hi = min(c.n, lo + run);
     u64 sum = 0, tied = tie_pre[q];
+#pragma unroll 2
     for (int i = lo; i < hi; i += 32) sum += drawn(i + lane, hi, tied);
     sum = warp_sum(sum);
     if (lane == 0) sh.sub[4 * warp + q] = sum;
   }
   if (tid == 0) sh.run_at = -1;
   __syncthreads();
-  u64 part[4] = {0, 0, 0, 0}, mine = 0, upto = 0;
+  constexpr int kPer = kSubs / 32;
+  u64 part[kPer] = {}, mine = 0, upto = 0;
   if (warp == 0) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      part[q] = sh.sub[4 * lane + q];
+    for (int q = 0; q < kPer; ++q) {
+      part[q] = sh.sub[kPer * lane + q];
       mine += part[q];
     }
     upto = warp_prefix(mine);
@@ -732,9 +798,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
   if (warp == 0) {  // the run that holds the target
     u64 at = before + upto - mine;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < kPer; ++q) {
       if (at <= target && target < at + part[q]) {
-        sh.run_at = 4 * lane + q;
+        sh.run_at = kPer * lane + q;
         sh.run_sum = at;
       }
       at += part[q];
@@ -763,15 +829,15 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Params p) {
 template <typename T>
 static hxm_status launch(Params p, int rows, cudaStream_t st) {
   typedef typename Key<T>::type K;
-  // CTAs per row: as many as keep the keys within shared memory, more while the SMs are not full
-  // (a row then goes through fewer tokens per thread)
-  const int most = (int)(200 * 1024 / sizeof(K));
+  // CTAs per row: as many as leave room for two on an SM (92 KB of keys each; 8 CTAs reach 2^18 tokens
+  // of 32 bits with one on an SM), more while that leaves SMs idle: a thread then has fewer tokens
   int cl = 1;
-  while ((p.vocab + cl - 1) / cl > most) cl *= 2;
-  while (cl < 8 && (int64_t)rows * cl * 2 <= 148 && p.vocab / cl > 4 * kThreads) cl *= 2;
+  while (cl < 8 && (size_t)((p.vocab + cl - 1) / cl) * sizeof(K) > 92 * 1024) cl *= 2;
+  while (cl < 8 && (int64_t)rows * cl * 2 <= 2 * 148 && p.vocab / cl > 4 * kThreads) cl *= 2;
   p.slice = ((p.vocab + cl - 1) / cl + 7) / 8 * 8;
   const size_t smem = kRegion + (size_t)p.slice * sizeof(K);
   HXM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  HXM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cl));
   cfg.blockDim = dim3(kThreads);
