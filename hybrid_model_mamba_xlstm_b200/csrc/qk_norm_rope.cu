@@ -9,8 +9,7 @@
 // pairs, the gradients are g = R^T dy, dw = sum over rows of g * n, and
 //   dx = (w g - n mean(w g n)) / sqrt(mean x^2 + eps).
 // The angle positions * base^(-2p/rotary) is formed in 64 bits, in turns, and only its fraction goes
-// to 32 bits: at position 10^6 a 32-bit angle would be off by 0.06.  The cosines and sines of a token
-// are made once for all of its heads, in shared memory.
+// to 32 bits: at position 10^6 a 32-bit angle would be off by 0.06.
 #include "capi_internal.h"
 #include "common.cuh"
 
@@ -57,88 +56,33 @@ HXM_DEV void angles(const Params& p, int64_t tok0, int nt, float2* cs) {
   }
 }
 
-template <typename T, int V>
-HXM_DEV void load_vec(const T* p, float (&v)[V]) {
-  static_assert(V * sizeof(T) == 16, "16-byte vectors");
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = to_f32<T>(e[j]);
-}
-template <typename T, int V>
-HXM_DEV void store_vec(T* p, const float (&v)[V]) {
-  uint4 raw;
-  T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-  for (int j = 0; j < V; ++j) e[j] = from_f32<T>(v[j]);
-  *reinterpret_cast<uint4*>(p) = raw;
-}
+// How a lane holds its V elements of a row, and which of them are pairs.
+enum Mode : int {
+  kHalves = 0,  // V/2 elements from each half of the row: pairs (j, j + V/2); the whole row is rotated
+  kRun = 1,     // V elements in a row: pairs (2j, 2j + 1), those behind `rotary` turn by 0
+};
 
-// Turns this lane's vectors by sign * angle.  Lane `gl` of a row's G lanes holds vectors gl, gl + G, ..
-// (NV of them); pairs of the half-split form sit in vectors half/V apart, fetched by shuffle.
-template <int V, int NV>
-HXM_DEV void rotate(float (&y)[NV][V], const Params& p, const float2* cs, int gl, int G, float sign) {
-  if (p.rotary == 0) return;
-  if (p.interleaved) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + gl) * V;
-#pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        if (c + j < p.rotary) {
-          const float2 t = cs[(c + j) >> 1];
-          const float s = sign * t.y, a = y[i][j], b = y[i][j + 1];
-          y[i][j] = a * t.x - b * s;
-          y[i][j + 1] = b * t.x + a * s;
-        }
-      }
-    }
-    return;
-  }
-  const int half = p.rotary / 2, hv = half / V;  // half is a multiple of V on this path
-  float other[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int vi = i * G + gl;
-    const int pv = vi < hv ? vi + hv : (vi < 2 * hv ? vi - hv : vi);
-    const int src = ((threadIdx.x & 31) & ~(G - 1)) + (pv & (G - 1));
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float r = __shfl_sync(0xffffffffu, y[0][j], src);
-#pragma unroll
-      for (int m = 1; m < NV; ++m) {
-        const float t = __shfl_sync(0xffffffffu, y[m][j], src);
-        if (pv / G == m) r = t;
-      }
-      other[i][j] = r;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int vi = i * G + gl;
-    if (vi < 2 * hv) {
-      const bool first = vi < hv;
-      const float2* t = cs + (first ? vi : vi - hv) * V;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float s = sign * t[j].y;
-        y[i][j] = first ? y[i][j] * t[j].x - other[i][j] * s : y[i][j] * t[j].x + other[i][j] * s;
-      }
-    }
-  }
-}
-
-// Rows whose vectors fit the registers of G <= 32 lanes: dim a multiple of the 16-byte vector, NV
-// vectors a lane.  A block takes tokens_per_block tokens with all of their heads; 256 / G rows at once.
-template <typename T, int G, int NV, bool BWD>
+// Rows that fit the registers of G <= 32 lanes, NV * 16 bytes a lane.  A group of G lanes takes one token
+// and every (256 / G / tokens_per_block)-th of its heads, so a lane's cosines and sines serve all of its
+// rows; R rows are loaded before the first is worked on, for the latency of HBM.
+template <typename T, int G, int NV, int MODE, bool BWD>
 __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), H = V / 2, R = NV > 1 ? 2 : (BWD ? 2 : 4);
   extern __shared__ __align__(16) unsigned char shraw[];
-  float2* cs = reinterpret_cast<float2*>(shraw);
+  double* freq = reinterpret_cast<double*>(shraw);  // turns per position of each pair
+  const int half = p.rotary / 2;
   const int gl = threadIdx.x & (G - 1), group = threadIdx.x / G;
   constexpr int kGroups = kThreads / G;
+  const int it = group & (p.tokens_per_block - 1), h0 = group / p.tokens_per_block, hs = kGroups / p.tokens_per_block;
   const int64_t tokens = (int64_t)p.batch * p.seqlen;
-  const int half = p.rotary / 2;
+  for (int i = threadIdx.x; i < half; i += kThreads)
+    freq[i] = exp2(-2.0 * i / p.rotary * p.log2_base) * 0.15915494309189535;
+  __syncthreads();
+  // column of element j of this lane's vector i
+  auto col = [&](int i, int j) {
+    return MODE == kHalves ? (i * G + gl) * H + (j < H ? j : j - H + p.dim / 2) : (i * G + gl) * V + j;
+  };
+  const bool has[2] = {gl * V < p.dim, NV > 1 && (G + gl) * V < p.dim};  // dim is a multiple of V
   float dw[2][NV][V];
   if (BWD) {
 #pragma unroll
@@ -148,88 +92,127 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[s][i][j] = 0.f;
   }
-  for (int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block; tok0 < tokens; tok0 += (int64_t)gridDim.x * p.tokens_per_block) {
-    const int nt = (int)min((int64_t)p.tokens_per_block, tokens - tok0);
-    if (half) {
-      __syncthreads();
-      angles(p, tok0, nt, cs);
-      __syncthreads();
+  auto load = [&](const T* row, int i) {
+    if (MODE == kRun) return *reinterpret_cast<const uint4*>(row + (i * G + gl) * V);
+    const uint2 a = *reinterpret_cast<const uint2*>(row + (i * G + gl) * H);
+    const uint2 b = *reinterpret_cast<const uint2*>(row + p.dim / 2 + (i * G + gl) * H);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  };
+  auto store = [&](T* row, int i, const float (&v)[V]) {
+    uint4 raw;
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < V; ++j) e[j] = from_f32<T>(v[j]);
+    if (MODE == kRun) {
+      *reinterpret_cast<uint4*>(row + (i * G + gl) * V) = raw;
+    } else {
+      *reinterpret_cast<uint2*>(row + (i * G + gl) * H) = make_uint2(raw.x, raw.y);
+      *reinterpret_cast<uint2*>(row + p.dim / 2 + (i * G + gl) * H) = make_uint2(raw.z, raw.w);
     }
+  };
+  for (int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block; tok0 < tokens; tok0 += (int64_t)gridDim.x * p.tokens_per_block) {
+    const int64_t tok = tok0 + it;
+    const bool here = tok < tokens;
+    const int64_t b = here ? tok / p.seqlen : 0, t = here ? tok - b * p.seqlen : 0;
+    float2 cs[NV][H];
+    if (half) {
+      const int64_t at = here ? p.pos[b * p.spos[0] + t * p.spos[1]] : 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const int pr = (i * G + gl) * H + j;
+          const double turns = (double)at * freq[pr < half ? pr : 0];
+          float sn, c;
+          sincospif((float)(2.0 * (turns - rint(turns))), &sn, &c);
+          cs[i][j] = pr < half ? make_float2(c, sn) : make_float2(1.f, 0.f);
+        }
+    }
+    auto turn = [&](float (&y)[V], int i, float sign) {
+      if (!half) return;
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        float &u = y[MODE == kHalves ? j : 2 * j], &v = y[MODE == kHalves ? j + H : 2 * j + 1];
+        const float c = cs[i][j].x, sn = sign * cs[i][j].y, a = u;
+        u = a * c - v * sn;
+        v = v * c + a * sn;
+      }
+    };
 #pragma unroll
     for (int sd = 0; sd < 2; ++sd) {
       const Side& s = p.s[sd];
-      const int rows = nt * s.heads;
       float w[NV][V];
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = (i * G + gl) * V + j;
-          w[i][j] = c < p.dim ? (s.w ? s.w[c] : 1.f) : 0.f;
-        }
+        for (int j = 0; j < V; ++j) w[i][j] = s.w && has[i] ? s.w[col(i, j)] : 1.f;
+      const T* xt = static_cast<const T*>(s.x) + b * s.sx[0] + t * s.sx[1];
+      const T* gt = BWD ? static_cast<const T*>(s.g) + b * s.sg[0] + t * s.sg[1] : nullptr;
+      T* ot = static_cast<T*>(s.out) + b * s.so[0] + t * s.so[1];
       // every lane of the warp goes through the loop (the shuffles need them all)
-      for (int r0 = 0; r0 < rows; r0 += kGroups) {
-        const int r = r0 + group;
-        const bool live = r < rows;
-        const int it = live ? r / s.heads : 0, h = live ? r % s.heads : 0;
-        const int64_t tok = tok0 + it, b = tok / p.seqlen, t = tok % p.seqlen;
-        float x[NV][V];
-        float ssq = 0.f;
-        const T* xr = static_cast<const T*>(s.x) + b * s.sx[0] + t * s.sx[1] + h * s.sx[2];
+      for (int hb = 0; hb < s.heads; hb += R * hs) {
+        uint4 xr[R][NV], gr[R][NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * G + gl) * V;
-#pragma unroll
-          for (int j = 0; j < V; ++j) x[i][j] = 0.f;
-          if (live && c < p.dim) load_vec<T, V>(xr + c, x[i]);
-#pragma unroll
-          for (int j = 0; j < V; ++j) ssq = fmaf(x[i][j], x[i][j], ssq);
-        }
-        float g[NV][V];
-        if (BWD) {
-          const T* gr = static_cast<const T*>(s.g) + b * s.sg[0] + t * s.sg[1] + h * s.sg[2];
+        for (int r = 0; r < R; ++r) {
+          const int h = hb + r * hs + h0;
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + gl) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) g[i][j] = 0.f;
-            if (live && c < p.dim) load_vec<T, V>(gr + c, g[i]);
+            const bool live = here && h < s.heads && has[i];
+            xr[r][i] = live ? load(xt + h * s.sx[2], i) : make_uint4(0, 0, 0, 0);
+            if (BWD) gr[r][i] = live ? load(gt + h * s.sg[2], i) : make_uint4(0, 0, 0, 0);
           }
         }
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-        const float inv = rsqrtf(ssq / (float)p.dim + p.eps);
-        T* orow = static_cast<T*>(s.out) + b * s.so[0] + t * s.so[1] + h * s.so[2];
-        if (!BWD) {
+        for (int r = 0; r < R; ++r) {
+          const int h = hb + r * hs + h0;
+          if (hb + r * hs >= s.heads) break;  // block-uniform
+          float x[NV][V], ssq = 0.f;
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i][j] = x[i][j] * inv * w[i][j];
-          rotate<V, NV>(x, p, cs + it * half, gl, G, 1.f);
-        } else {
-          rotate<V, NV>(g, p, cs + it * half, gl, G, -1.f);
-          float m = 0.f;
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
+          for (int i = 0; i < NV; ++i) {
+            const T* e = reinterpret_cast<const T*>(&xr[r][i]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              x[i][j] *= inv;
-              const float gn = g[i][j] * x[i][j];
-              if (live) dw[sd][i][j] += gn;
-              m = fmaf(gn, w[i][j], m);
+              x[i][j] = to_f32<T>(e[j]);
+              ssq = fmaf(x[i][j], x[i][j], ssq);
+            }
+          }
+#pragma unroll
+          for (int o = G / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+          const float inv = rsqrtf(ssq / (float)p.dim + p.eps);
+          if (!BWD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+              for (int j = 0; j < V; ++j) x[i][j] = x[i][j] * inv * w[i][j];
+              turn(x[i], i, 1.f);
+            }
+          } else {
+            float g[NV][V], m = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+              const T* e = reinterpret_cast<const T*>(&gr[r][i]);
+#pragma unroll
+              for (int j = 0; j < V; ++j) g[i][j] = to_f32<T>(e[j]);
+              turn(g[i], i, -1.f);
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                x[i][j] *= inv;
+                const float gn = g[i][j] * x[i][j];
+                dw[sd][i][j] += gn;  // 0 where this lane has no row
+                m = fmaf(gn, w[i][j], m);
+              }
             }
 #pragma unroll
-          for (int o = G / 2; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-          m /= (float)p.dim;
+            for (int o = G / 2; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+            m /= (float)p.dim;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+              for (int j = 0; j < V; ++j) x[i][j] = inv * (w[i][j] * g[i][j] - x[i][j] * m);
+          }
 #pragma unroll
           for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[i][j] = inv * (w[i][j] * g[i][j] - x[i][j] * m);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int c = (i * G + gl) * V;
-          if (live && c < p.dim) store_vec<T, V>(orow + c, x[i]);
+            if (here && h < s.heads && has[i]) store(ot + h * s.so[2], i, x[i]);
         }
       }
     }
@@ -241,11 +224,9 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < NV; ++i)
+        if (has[i])
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = (i * G + gl) * V + j;
-          if (c < p.dim) red[group * p.dim + c] = dw[sd][i][j];
-        }
+          for (int j = 0; j < V; ++j) red[group * p.dim + col(i, j)] = dw[sd][i][j];
       __syncthreads();
       for (int c = threadIdx.x; c < p.dim; c += kThreads) {
         float a = 0.f;
@@ -358,30 +339,37 @@ constexpr int kSMs = 148;
 // Blocks whose weight sums the gradients keep: four per SM.
 constexpr int kBwdBlocks = 4 * kSMs;
 
-template <typename T, int G, int NV, bool BWD>
-static hxm_status launch_vec(Params& p, cudaStream_t st) {
+template <typename T, int G, int NV, int MODE, bool BWD>
+static hxm_status launch_mode(Params& p, cudaStream_t st) {
   const int64_t tokens = (int64_t)p.batch * p.seqlen;
-  // tokens a block takes at once: more share the angles' latency, fewer fill the SMs
-  int64_t tpb = tokens / (kSMs * 8);
-  p.tokens_per_block = (int)(tpb < 1 ? 1 : (tpb > 8 ? 8 : tpb));
-  int64_t grid = (tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  if (BWD && grid > kBwdBlocks) grid = kBwdBlocks;
-  if (grid > 0x7fffffff) grid = 0x7fffffff;
-  size_t smem = (size_t)p.tokens_per_block * (p.rotary / 2) * sizeof(float2);
+  // tokens a block takes at once: one while blocks are few, for their number; up to 8 (every group keeps
+  // some heads), so that a lane's angles serve more rows
+  int tpb = 1;
+  while (tpb < 8 && tpb * 2 <= kThreads / G && tokens / (tpb * 2) >= 4 * kSMs) tpb *= 2;
+  p.tokens_per_block = tpb;
+  int64_t grid = (tokens + tpb - 1) / tpb;
+  if (grid > 16 * kSMs) grid = 16 * kSMs;  // the pairs' frequencies are made once a block
+  size_t smem = (size_t)(p.rotary / 2) * sizeof(double);
   if (BWD) {
     const size_t red = (size_t)(kThreads / G) * p.dim * sizeof(float);
     if (red > smem) smem = red;
     // blocks that take no token write zeros: the join always reads kBwdBlocks sums
     grid = kBwdBlocks;
   }
-  vec_kernel<T, G, NV, BWD><<<(unsigned)grid, kThreads, smem, st>>>(p);
+  vec_kernel<T, G, NV, MODE, BWD><<<(unsigned)grid, kThreads, smem, st>>>(p);
   return check_launch("hxm_qk_norm_rope");
+}
+
+template <typename T, int G, int NV, bool BWD>
+static hxm_status launch_vec(Params& p, cudaStream_t st) {
+  return p.rotary == 0 || p.interleaved ? launch_mode<T, G, NV, kRun, BWD>(p, st) : launch_mode<T, G, NV, kHalves, BWD>(p, st);
 }
 
 template <typename T, bool BWD>
 static hxm_status launch(Params& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  bool vec = p.dim % V == 0 && p.dim <= 64 * V && (p.interleaved || (p.rotary / 2) % V == 0);
+  // the register kernel: whole vectors, and halves that are rotated entirely or not at all
+  bool vec = p.dim % V == 0 && p.dim <= 64 * V && (p.interleaved || p.rotary == 0 || p.rotary == p.dim);
   for (int i = 0; i < 2; ++i) {
     const Side& s = p.s[i];
     auto ok = [&](const void* ptr, const int64_t* st3) {
