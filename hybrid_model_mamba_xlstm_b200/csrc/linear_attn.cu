@@ -217,11 +217,13 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Segments: the recurrence is sequential in time, so a call with fewer CTAs than SMs is cut along
 // time; every segment but the last first sums its own k v^T (pass one), the others' sums are joined
-// when a segment starts.
-static void set_segments(Common& c, int64_t ctas, int chunk) {
+// when a segment starts.  Pass one and the joining cost about half a chunk's and a few chunks' time on
+// the tensor cores, so a segment has `least` chunks there (4); on the FP32 pipe a chunk takes so much
+// longer that one will do (2 x 513 x 4 heads of 64, fp32: 170 us uncut).
+static void set_segments(Common& c, int64_t ctas, int chunk, int least) {
   const int chunks = ceil_div(c.seqlen, chunk);
   int64_t want = ctas > 0 ? kSMs / ctas : 1;
-  if (want > chunks / 4) want = chunks / 4;
+  if (want > chunks / least) want = chunks / least;
   if (want < 2) want = 1;
   c.seg_len = (int)(ceil_div(chunks, want) * (int64_t)chunk);
   c.nseg = c.seqlen > 0 ? ceil_div(c.seqlen, c.seg_len) : 1;
@@ -306,7 +308,8 @@ static bool plan(Common& c, const Problem* p, int np, hxm_dtype io) {
   int64_t ctas = 0;
   for (int i = 0; i < np; ++i) tc = tc && tc_ok(p[i], c.seqlen, io);
   for (int i = 0; i < np; ++i) ctas += (int64_t)c.batch * c.heads * ceil_div(p[i].dv, tc ? 64 : kTileV);
-  set_segments(c, ctas, 128);
+  if (tc) set_segments(c, ctas, 128, 4);
+  else set_segments(c, ctas, 64, 1);
   return tc;
 }
 

@@ -43,7 +43,7 @@ struct Common {
   int batch, heads, seqlen;
   const float* log_decay;
   const int32_t* lengths;
-  int nseg, seg_len;  // time segments of seg_len steps (a multiple of 128) in processing order
+  int nseg, seg_len;  // time segments of seg_len steps (whole chunks) in processing order
   int* error_flag;
   long long wait_limit;
 };
