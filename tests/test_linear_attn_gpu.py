@@ -85,6 +85,14 @@ def test_forward(ops, shape, dtype):
     check_forward(ops, q, k, v, ld, s0, dk ** -0.5)
 
 
+@pytest.mark.parametrize("dims", [(1, 2048, 40, 128, 128), (5, 1100, 32, 128, 128), (3, 900, 30, 64, 64), (2, 700, 40, 192, 128)])
+def test_many_heads_and_chunks(ops, dims):
+    """bf16 grids of more CTAs than the GPU has SMs, and many chunks per CTA, with a state on both sides."""
+    B, L, H, dk, dv = dims
+    q, k, v, ld, s0 = inputs(B, L, H, dk, dv, BF, seed=H, s0=True)
+    check_forward(ops, q, k, v, ld, s0, dk ** -0.5)
+
+
 @pytest.mark.parametrize("dtype,dk", [(F32, 64), (BF, 64), (BF, 192), (BF, 20)])
 def test_lengths_and_what_lies_behind_them(ops, dtype, dk):
     """Rows of length 0, 1, a chunk's edge and all; NaN and infinity behind each row's end change nothing, and
