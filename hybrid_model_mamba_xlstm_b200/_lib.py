@@ -427,4 +427,6 @@ def check(fn: str, status: int):
 def call(fn: str, args, stream: int = 0):
     """Call an hxm entry point with an args struct on `stream` (raw cudaStream_t)."""
     args.struct_size = ct.sizeof(args)
-    check(fn, getattr(lib(), fn)(ct.byref(args), ct.c_void_p(stream)))
+    status = getattr(_lib or lib(), fn)(ct.byref(args), stream)
+    if status != HXM_OK:
+        check(fn, status)

@@ -13,7 +13,7 @@
 // products of the output apart, O2 taking its factor g^i at the end.
 // Roundings to bf16: P and the copy of X that multiplies Q, one operand of each product of the bf16
 // output.  X itself, which is returned in fp32, comes from products that are exact to 32 bits: k is bf16
-// already, and a scaled V value is carried in three bf16 parts (two leave 2.8e-6, by measurement).
+// already, and a scaled V value is carried in three bf16 parts, which leave 2^-24 of it (two would leave up to 2^-16).
 //
 // Work is cut by role, so that the tensor core always has something queued while one chunk's
 // element-wise work runs: warps 0-7 (group A) turn S into P and write the output; warps 8-23 (group B)

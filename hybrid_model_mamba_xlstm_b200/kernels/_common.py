@@ -31,7 +31,13 @@ def require_cuda(*tensors, who: str):
     return dev
 
 
+# The raw cudaStream_t of a device's current stream: the Stream object around it costs 2 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -50,6 +56,12 @@ def on_device(device):
     """A context in which ``device`` is the current CUDA device (launches go to the current device's
     context, whatever stream they name); free when it already is."""
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def once_only(who):
+    """Raises in a backward that is itself being differentiated (create_graph=True): its kernels record nothing."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: its gradient cannot be differentiated again")
 
 
 def ptr(t):

@@ -13,7 +13,7 @@ import math
 import torch
 
 from .. import _lib
-from ._common import dtype_code, on_device, ptr, require_cuda, stream_of
+from ._common import dtype_code, on_device, once_only, ptr, require_cuda, stream_of
 
 __all__ = ["linear_attention", "linear_attention_bwd", "linear_attention_step"]
 
@@ -150,25 +150,27 @@ def linear_attention_bwd(q, k, v, log_decay, dout, *, scale=None, lengths=None, 
 
 class LinearAttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, s0, log_decay, scale, lengths, want_state):
+    def forward(ctx, q, k, v, s0, log_decay, scale, lengths, want_state, error_flag, wait_limit_cycles):
         ctx.save_for_backward(q, k, v, s0, log_decay, lengths)
-        ctx.scale = scale
-        out, sT = _forward(q, k, v, log_decay, scale, lengths, s0, want_state)
+        ctx.rest = (scale, error_flag, wait_limit_cycles)
+        out, sT = _forward(q, k, v, log_decay, scale, lengths, s0, want_state, error_flag, wait_limit_cycles)
         ctx.set_materialize_grads(False)
         return out, sT
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dsT):
+        once_only("linear_attention")
         q, k, v, s0, log_decay, lengths = ctx.saved_tensors
         if dout is None and dsT is None:
-            return (None,) * 8
+            return (None,) * 10
+        scale, error_flag, wait_limit_cycles = ctx.rest
         if dout is None:
             dout = torch.zeros(v.shape, device=v.device, dtype=v.dtype)
-        dq, dk, dv, ds0 = linear_attention_bwd(q, k, v, log_decay, dout.to(q.dtype), scale=ctx.scale, lengths=lengths,
+        dq, dk, dv, ds0 = linear_attention_bwd(q, k, v, log_decay, dout.to(q.dtype), scale=scale, lengths=lengths,
                                                initial_state=s0, d_final_state=dsT,
-                                               need_d_initial_state=s0 is not None and ctx.needs_input_grad[3])
-        return dq, dk, dv, ds0 if ds0 is None else ds0.to(s0.dtype), None, None, None, None
+                                               need_d_initial_state=s0 is not None and ctx.needs_input_grad[3],
+                                               error_flag=error_flag, wait_limit_cycles=wait_limit_cycles)
+        return (dq, dk, dv, ds0 if ds0 is None else ds0.to(s0.dtype)) + (None,) * 6
 
 
 def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_state=None, return_final_state=False,
@@ -185,8 +187,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
 
     dk <= 512, and dv <= 512 for gradients.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
     dv <= 256 too) runs on the tensor cores; everything else on the FP32 pipe.  error_flag: a device int32
-    tensor set to 1 if a bounded device wait gave up (the outputs are then not valid); wait_limit_cycles:
-    that bound in SM cycles (0: about 2 s)."""
+    tensor set to 1 if a bounded device wait of the call or of its gradients gave up (the outputs are then
+    not valid); wait_limit_cycles: that bound in SM cycles (0: about 2 s)."""
     who = "linear_attention"
     if q.dim() != 4:
         raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
@@ -195,7 +197,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
         if v.shape[-1] > 512:
             raise ValueError(f"{who}: gradients need dv <= 512, got {v.shape[-1]}")
         _decay(who, log_decay, q.shape[2])
-        out, sT = LinearAttentionFunction.apply(q, k, v, initial_state, log_decay, scale, lengths, bool(return_final_state))
+        out, sT = LinearAttentionFunction.apply(q, k, v, initial_state, log_decay, scale, lengths, bool(return_final_state),
+                                                error_flag, wait_limit_cycles)
     else:
         out, sT = _forward(q, k, v, log_decay, scale, lengths, initial_state, return_final_state, error_flag,
                            wait_limit_cycles)
@@ -228,8 +231,9 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
         ld = _decay(who, log_decay, nh)
         if out is None:
             out = torch.empty(bsz, nh, dv, device=dev, dtype=q.dtype)
-        elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1):
-            raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride")
+        elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1) or any(
+                s == 0 for s, n in zip(out.stride(), out.shape) if n > 1):
+            raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride and no repeated rows")
         a = _lib.LinearAttnStepArgs()
         a.batch, a.heads, a.dk, a.dv = bsz, nh, dk, dv
         a.io_dtype = dtype_code(q)

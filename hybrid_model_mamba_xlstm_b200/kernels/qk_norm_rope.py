@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from ._common import dtype_code, f32_param, on_device, ptr, require_cuda, stream_of
+from ._common import dtype_code, f32_param, on_device, once_only, ptr, require_cuda, stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_bwd"]
 
@@ -109,8 +109,8 @@ class QkNormRopeFunction(torch.autograd.Function):
         return _forward(q, k, qw, kw, positions, base, rotary, interleaved, eps)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
+        once_only("qk_norm_rope")
         q, k, qw, kw, positions = ctx.saved_tensors
         base, rotary, interleaved, eps = ctx.rest
         weights = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
