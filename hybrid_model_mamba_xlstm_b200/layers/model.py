@@ -14,6 +14,7 @@ from typing import List, Optional
 import torch
 import torch.nn as nn
 
+from ..kernels.sample import sample_tokens
 from .blocks import HybridBlock, RMSNorm
 
 
@@ -226,14 +227,29 @@ class HybridLanguageModel(nn.Module):
         return torch.cat(outs, dim=1)
 
     @torch.no_grad()
-    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None, cuda_graph=True):
+    def generate(self, input_ids, max_new_tokens=100, temperature=1.0, top_k=None, top_p=None, cuda_graph=True,
+                 min_p=None, uniforms=None):
         """Autoregressive sampling with the reference's interface and sampling rule
         (hybrid_xmamba/models/hybrid_lm.py:211-267), but one prefill over the
         prompt and then one single-token step per new token on the carried
         recurrent states, instead of re-running the whole prefix per token.
         With ``cuda_graph`` the single-token step (a few hundred small kernel
-        launches) is captured once and replayed (:class:`GraphDecoder`)."""
+        launches) is captured once and replayed (:class:`GraphDecoder`).
+
+        With ``min_p`` or ``uniforms`` (batch, max_new_tokens; fp32 in [0, 1)) the
+        tokens come from :func:`kernels.sample_tokens` instead, one launch per
+        token and one uniform number per token (drawn here where none are given);
+        ``temperature`` 0 is then greedy, and each setting may be a (batch,) tensor.
+        Equal logits at the top-k border then stay by rising token, where the
+        reference's rule keeps all of them."""
         self.eval()
+        kernel = min_p is not None or uniforms is not None
+        if kernel and uniforms is None:
+            uniforms = torch.rand(input_ids.shape[0], max_new_tokens, device=input_ids.device)
+        if kernel and uniforms.shape != (input_ids.shape[0], max_new_tokens):
+            raise ValueError(f"generate: uniforms must be {(input_ids.shape[0], max_new_tokens)}, got {tuple(uniforms.shape)}")
+        if kernel:
+            uniforms = uniforms.float().t().contiguous()  # a token's numbers side by side
         if cuda_graph and input_ids.is_cuda and max_new_tokens > 1:
             dec = GraphDecoder(self, input_ids.shape[0], input_ids.device)
             logits = dec.prefill(input_ids)[:, -1, :]
@@ -244,6 +260,14 @@ class HybridLanguageModel(nn.Module):
             step = lambda t: self.forward(t, caches=caches)
         out = [input_ids]
         for i in range(max_new_tokens):
+            if kernel:
+                # a row without any logit (NaN throughout) gives -1: token 0 goes on, an index all the same
+                nxt = sample_tokens(logits, uniforms[i], temperature=temperature, top_k=top_k, top_p=top_p,
+                                    min_p=min_p).clamp_(min=0)[:, None]
+                out.append(nxt)
+                if i + 1 < max_new_tokens:
+                    logits = step(nxt)[:, -1, :]
+                continue
             next_token_logits = logits.float() / temperature
             if top_k is not None:
                 kth = torch.topk(next_token_logits, top_k)[0][..., -1, None]

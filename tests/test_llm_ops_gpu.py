@@ -1,0 +1,233 @@
+"""The query / key norms with rotation, linear attention and sampling in one run, as a decoder uses them; linear
+attention's bounded waits; what the wrappers refuse of CUDA tensors; generate on sample_tokens.
+
+Tolerance of the fp32 runs: an element of q or k comes from a sum of d squares and some ten operations, a sum of the
+attention from at most L + dk + dv terms, each with a relative error of 2^-24: (L + dk + dv + 2 d + 64) 2^-24 times
+the same sum over absolute values (two norms, hence 2 d).
+"""
+import math
+
+import pytest
+import torch
+
+from tests.test_linear_attn_gpu import inputs, recur
+from tests.test_sample_gpu import ref_row
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs CUDA")
+    torch.cuda.set_device(0)
+    from hybrid_model_mamba_xlstm_b200 import kernels
+    return kernels
+
+
+def norm_rope(x, w, pos, base=1e4, eps=1e-6):
+    """Plain form in 64 bits, halves as pairs."""
+    x, d = x.double(), x.shape[-1]
+    y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * w.double()
+    a = pos.double()[..., None, None] * base ** (-torch.arange(0, d, 2, device=x.device, dtype=torch.float64) / d)
+    lo, hi = y[..., :d // 2], y[..., d // 2:]
+    return torch.cat([lo * a.cos() - hi * a.sin(), hi * a.cos() + lo * a.sin()], -1)
+
+
+def test_a_decoders_prompt_and_steps(ops):
+    """Token -> q, k, v (a table) -> norms and rotation -> attention over a padded batch of prompts -> logits ->
+    tokens, then steps on the carried states, all positions a row's own.  Each attention output is held to the
+    64-bit recurrence over the row's whole history, each token to the sampling rule on the logits."""
+    B, L, H, d, V, steps = 3, 70, 2, 64, 50, 6
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    table, out_w = r(V, 3 * H * d), r(H * d, V) / (H * d) ** 0.5
+    qw, kw, ld = 1 + 0.1 * r(d), 1 + 0.1 * r(d), torch.tensor([-0.02, -0.3], device="cuda")
+    lengths = torch.tensor([70, 1, 33], device="cuda")
+    ids = torch.randint(0, V, (B, L), generator=g, device="cuda")
+    u = torch.rand(B, steps, generator=g, device="cuda")
+
+    def heads(t):
+        return (x.unflatten(-1, (H, d)) for x in table[t].chunk(3, -1))
+
+    q, k, v = heads(ids)
+    q, k = ops.qk_norm_rope(q, k, qw, kw, torch.arange(L, device="cuda"))
+    o, state = ops.linear_attention(q, k, v, ld, lengths=lengths, return_final_state=True)
+    last = o[torch.arange(B, device="cuda"), lengths - 1]
+    history = [ids[b, :int(lengths[b])] for b in range(B)]
+    for i in range(steps):
+        for b in range(B):
+            q, k, v = (x.double()[None] for x in heads(history[b]))
+            at = torch.arange(len(history[b]), device="cuda")[None]
+            q, k = norm_rope(q, qw, at), norm_rope(k, kw, at)
+            ref = recur(q, k, v, ld, d ** -0.5)[0][0, -1]
+            A = recur(q.abs(), k.abs(), v.abs(), ld, d ** -0.5)[0][0, -1]
+            # a rotated element is a sum of two: its error is relative to their absolute values
+            A = A.amax() * 2
+            assert bool(((last[b].double() - ref).abs() <= (len(history[b]) + 4 * d + 64) * 2.0 ** -24 * A).all())
+        logits = (last.flatten(1).double() @ out_w.double()).float()
+        tokens = ops.sample_tokens(logits, u[:, i], temperature=0.7, top_k=20, top_p=0.9, min_p=0.01)
+        for b in range(B):
+            t, _, near = ref_row(logits[b].double().cpu().numpy(), float(u[b, i]), float(torch.tensor(0.7)), 20,
+                                 float(torch.tensor(0.9)), float(torch.tensor(0.01)))
+            assert near < V * 2.0 ** -45 or int(tokens[b]) == t
+            history[b] = torch.cat([history[b], tokens[b:b + 1]])
+        q, k, v = heads(tokens)
+        q, k = ops.qk_norm_rope(q[:, None], k[:, None], qw, kw, (lengths + i)[:, None])
+        last = ops.linear_attention_step(q[:, 0], k[:, 0], v, ld, state)
+
+
+def test_gradients_through_both(ops):
+    """Gradients of projections, norm weights and the first state through rotation and attention, against 64-bit
+    autograd of the plain forms.  Norm of the error: each of the T = L + dk + dv + 2 d + 64 roundings on the way of
+    an element is at most 2^-24 of a sum over absolute values, whose norm is below T times the result's."""
+    B, L, H, d = 2, 45, 2, 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    leaves = [r(B, L, 3 * H * d), 1 + 0.1 * r(d), 1 + 0.1 * r(d), r(B, H, d, d)]
+    ld, w, pos = torch.tensor([-0.02, -0.3], device="cuda"), r(B, L, H, d), torch.arange(L, device="cuda")
+
+    def run(leaves, plain):
+        x, qw, kw, s0 = leaves
+        q, k, v = (t.unflatten(-1, (H, d)) for t in x.chunk(3, -1))
+        if plain:
+            q, k = norm_rope(q, qw, pos), norm_rope(k, kw, pos)
+            return recur(q, k, v, ld, d ** -0.5, s0=s0)[0]
+        q, k = ops.qk_norm_rope(q, k, qw, kw, pos)
+        return ops.linear_attention(q, k, v, ld, initial_state=s0)
+
+    a = [t.clone().requires_grad_() for t in leaves]
+    b = [t.double().requires_grad_() for t in leaves]
+    got = torch.autograd.grad((run(a, False) * w).sum(), a)
+    ref = torch.autograd.grad((run(b, True) * w).sum(), b)
+    T = L + 4 * d + 64
+    for x, y in zip(got, ref):
+        assert float((x.double() - y).norm() / y.norm()) <= T * 2.0 ** -24
+
+
+@pytest.mark.parametrize("L,H,d", [(300, 2, 128), (300, 2, 192), (4000, 1, 64)])
+def test_attention_waits_run_out(ops, L, H, d):
+    """A negative limit makes every wait give up at once: the kernel drains its own loads, frees its tensor memory,
+    sets the word and returns, and the next call is as before (4000 steps of one head: cut along time)."""
+    q, k, v, ld, s0 = inputs(1, L, H, d, d, BF, seed=d, s0=True)
+    flag = torch.zeros(1, device="cuda", dtype=torch.int32)
+
+    def both(limit):
+        o, sT = ops.linear_attention(q, k, v, ld, initial_state=s0, return_final_state=True, error_flag=flag, wait_limit_cycles=limit)
+        return (o, sT) + ops.linear_attention_bwd(q, k, v, ld, v, initial_state=s0, error_flag=flag, wait_limit_cycles=limit)
+
+    first = both(0)
+    assert int(flag) == 0
+    both(-1)
+    torch.cuda.synchronize()
+    assert int(flag) == 1
+    flag.zero_()
+    again = both(0)
+    assert int(flag) == 0
+    for x, y in zip(first, again):
+        assert torch.equal(x, y)
+
+
+def test_attention_refusals(ops):
+    q, k, v, ld, s0 = inputs(2, 9, 2, 16, 24, F32, s0=True)
+    f, step = ops.linear_attention, ops.linear_attention_step
+    bad = [lambda: f(q[0], k, v, ld), lambda: f(q, k[:, :-1], v, ld), lambda: f(q, k, v[..., 0], ld), lambda: f(q, k, v, ld[:1]),
+           lambda: f(q, k, v, ld, scale=0.0), lambda: f(q, k, v, ld, scale=float("nan")), lambda: f(q, k, v, ld, scale=1e-60),
+           lambda: f(q, k, v, ld, lengths=torch.ones(3, device="cuda", dtype=torch.int32)),
+           lambda: f(q, k, v, ld, lengths=torch.ones(2, device="cuda")), lambda: f(q, k, v, ld, initial_state=s0[..., :-1]),
+           lambda: f(q, k, v, ld.clone().requires_grad_()),
+           lambda: f(q.clone().requires_grad_(), k, torch.zeros(2, 9, 2, 520, device="cuda"), ld),
+           lambda: ops.linear_attention_bwd(q, k, v, ld, v[:, :-1]), lambda: ops.linear_attention_bwd(q, k, v, ld, v, d_final_state=s0[:1]),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0[:1]), lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0.to(BF)),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0.transpose(2, 3).contiguous().transpose(2, 3)),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0[:1].expand(2, -1, -1, -1)),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0.clone().requires_grad_()),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out=torch.empty(2, 2, 16, device="cuda")),
+           lambda: step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out=torch.empty(1, 2, 24, device="cuda").expand(2, -1, -1))]
+    before = s0.clone()
+    for go in bad:
+        with pytest.raises(ValueError):
+            go()
+    for go in (lambda: f(q.half(), k.half(), v.half(), ld), lambda: f(q, k.to(BF), v, ld), lambda: step(q[:, 0], k[:, 0].to(BF), v[:, 0], ld, s0)):
+        with pytest.raises(TypeError):
+            go()
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        f(q, k, v, ld.cpu())
+    x = torch.zeros(1, 2, 1, 600, device="cuda")
+    with pytest.raises(Exception, match="at most 512"):
+        f(x, x, x, ld[:1])
+    leaf = q.clone().requires_grad_()
+    (gr,) = torch.autograd.grad(f(leaf, k, v, ld).sum(), leaf, create_graph=False)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(f(leaf, k, v, ld).sum(), leaf, create_graph=True)
+    assert torch.equal(s0, before)
+
+
+def test_norm_refusals(ops):
+    q, k = torch.randn(2, 5, 4, 32, device="cuda"), torch.randn(2, 5, 1, 32, device="cuda")
+    w, pos = torch.ones(32, device="cuda"), torch.arange(5, device="cuda")
+    f = ops.qk_norm_rope
+    bad = [lambda: f(q[0], k), lambda: f(q, k[:, :-1]), lambda: f(q, k[..., :-1]), lambda: f(q, k, w[:-1]), lambda: f(q, k, w, w[:-1]),
+           lambda: f(q, k, w, w, pos, rotary_dim=3), lambda: f(q, k, w, w, pos, rotary_dim=34), lambda: f(q, k, w, w, pos, rotary_dim=-2),
+           lambda: f(q, k, rotary_dim=8), lambda: f(q, k, w, w, pos.float()), lambda: f(q, k, w, w, pos[:-1]),
+           lambda: f(q, k, w, w, pos, rope_base=0.0), lambda: f(q, k, w, w, pos, rope_base=float("inf")),
+           lambda: ops.qk_norm_rope_bwd(q, k, w, w, q[:, :-1], k, pos)]
+    for go in bad:
+        with pytest.raises(ValueError):
+            go()
+    for go in (lambda: f(q.double(), k.double()), lambda: f(q, k.to(BF))):
+        with pytest.raises(TypeError):
+            go()
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        f(q, k, w.cpu())
+    leaf = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(f(leaf, k)[0].square().sum(), leaf, create_graph=True)
+
+
+def test_sampling_refusals(ops):
+    x, u = torch.randn(3, 40, device="cuda"), torch.rand(3, device="cuda")
+    f = ops.sample_tokens
+    bad = [lambda: f(x[0], u), lambda: f(x, u[:2]), lambda: f(x[:, :0], u), lambda: f(x, u, temperature=-1.0),
+           lambda: f(x, u, temperature=float("nan")), lambda: f(x, u, top_k=-1), lambda: f(x, u, top_k=1.5), lambda: f(x, u, top_p=1.1),
+           lambda: f(x, u, top_p=-0.1), lambda: f(x, u, min_p=2.0), lambda: f(x, u, min_p=float("nan")),
+           lambda: f(x, u, temperature=torch.ones(2, device="cuda")), lambda: f(x, u, top_p=torch.ones(3, 1, device="cuda"))]
+    for go in bad:
+        with pytest.raises(ValueError):
+            go()
+    for go in (lambda: f(x.double(), u), lambda: f(x, u, top_k=torch.ones(3, device="cuda"))):
+        with pytest.raises(TypeError):
+            go()
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        f(x, u.cpu())
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_generate_from_uniforms(ops, graph):
+    """The tokens of generate are sample_tokens' on the model's own logits, repeat exactly for the same numbers, and
+    are the largest logits' at temperature 0; without min_p and uniforms the sampling is as before."""
+    import hybrid_model_mamba_xlstm_b200.layers as layers
+    torch.manual_seed(0)
+    cfg = layers.HybridConfig(vocab_size=97, dim=64, num_layers=4, layer_pattern=["mamba", "mamba", "mlstm", "slstm"], state_size=16,
+                              conv_size=4, expand_factor=2, head_dim=32, num_heads=2, slstm_num_heads=4, dropout=0.0, slstm_recurrent=False)
+    model = layers.HybridLanguageModel(cfg).cuda().eval()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    prompt, u = torch.randint(0, 97, (2, 9), device="cuda", generator=g), torch.rand(2, 6, device="cuda", generator=g)
+    args = dict(max_new_tokens=6, temperature=0.8, top_k=30, top_p=0.95, cuda_graph=graph)
+    out = model.generate(prompt, min_p=0.02, uniforms=u, **args)
+    assert out.shape == (2, 15) and torch.equal(out[:, :9], prompt)
+    assert torch.equal(out, model.generate(prompt, min_p=0.02, uniforms=u, **args))
+    with torch.no_grad():  # the same pieces: prompt, then one token at a time
+        caches = model.init_caches()
+        logits = model(prompt, caches=caches)[:, -1, :]
+        for i in range(6):
+            t = ops.sample_tokens(logits, u[:, i], temperature=0.8, top_k=30, top_p=0.95, min_p=0.02)
+            assert torch.equal(t, out[:, 9 + i])
+            logits = model(t[:, None], caches=caches)[:, -1, :]
+    greedy = model.generate(prompt, max_new_tokens=6, temperature=0, uniforms=u, cuda_graph=graph)
+    assert torch.equal(greedy, model.generate(prompt, max_new_tokens=6, top_k=1, cuda_graph=graph))
+    drawn = model.generate(prompt, min_p=0.1, **args)
+    assert drawn.shape == (2, 15) and 0 <= int(drawn.min()) and int(drawn.max()) < 97
+    with pytest.raises(ValueError, match="uniforms"):
+        model.generate(prompt, max_new_tokens=6, uniforms=u[:, :5])
