@@ -361,37 +361,52 @@ struct StepParams {
 // S = g S + k v^T and out = scale S^T q for one token: the state is read and written once, 8 dk dv
 // bytes, which is all the time there is.  One CTA per (batch, head, 32 * VEC value columns); its
 // 8 warps share the dk rows, lane l holds VEC columns, and the warps' partial sums of the output
-// join in shared memory.
+// join in shared memory.  A warp has kRows rows on their way at once: 128 x 16 states of 128 x 128 take
+// 42 us, 6.3 TB/s (row by row, the store of one before the load of the next, 55 us).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) step_kernel(const StepParams p) {
+  constexpr int kRows = 8;
   const int h = blockIdx.y, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int e = (blockIdx.x * 32 + lane) * VEC;
-  const float g = (float)exp2((double)p.log_decay[h] * 1.4426950408889634);
   const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + h * p.sq[1];
   const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[1];
   const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[1];
-  float* s = p.s + b * p.ss[0] + h * p.ss[1];
+  float* s = p.s + b * p.ss[0] + h * p.ss[1] + e;
   __shared__ float part[8][32 * VEC];
   float acc[VEC] = {};
   if (e < p.dv) {
-    float vv[VEC];
+    for (int d0 = warp; d0 < p.dk; d0 += 8 * kRows) {
+      float x[kRows][VEC], kd[kRows], qd[kRows];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) vv[i] = to_f32<T>(v[e + i]);
-#pragma unroll 4
-    for (int d = warp; d < p.dk; d += 8) {
-      const float kd = to_f32<T>(k[d]), qd = to_f32<T>(q[d]);
-      float* row = s + d * p.ss[2] + e;
-      float x[VEC];
-      if (VEC == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row);
-      else x[0] = row[0];
+      for (int r = 0; r < kRows; ++r)
+        if (d0 + 8 * r < p.dk) {
+          const float* row = s + (d0 + 8 * r) * p.ss[2];
+          if (VEC == 4) *reinterpret_cast<float4*>(x[r]) = __ldcs(reinterpret_cast<const float4*>(row));
+          else x[r][0] = row[0];
+        }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        x[i] = fmaf(g, x[i], kd * vv[i]);
-        acc[i] = fmaf(qd, x[i], acc[i]);
+      for (int r = 0; r < kRows; ++r) {
+        const bool in = d0 + 8 * r < p.dk;
+        kd[r] = in ? to_f32<T>(k[d0 + 8 * r]) : 0.f;
+        qd[r] = in ? to_f32<T>(q[d0 + 8 * r]) : 0.f;
       }
-      if (VEC == 4) *reinterpret_cast<float4*>(row) = *reinterpret_cast<float4*>(x);
-      else row[0] = x[0];
+      const float g = (float)exp2((double)p.log_decay[h] * 1.4426950408889634);
+      float vv[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) vv[i] = to_f32<T>(v[e + i]);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if (d0 + 8 * r >= p.dk) continue;
+        float* row = s + (d0 + 8 * r) * p.ss[2];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          x[r][i] = fmaf(g, x[r][i], kd[r] * vv[i]);
+          acc[i] = fmaf(qd[r], x[r][i], acc[i]);
+        }
+        if (VEC == 4) __stcs(reinterpret_cast<float4*>(row), *reinterpret_cast<float4*>(x[r]));
+        else row[0] = x[r][0];
+      }
     }
   }
 #pragma unroll

@@ -58,7 +58,7 @@ HXM_DEV void angles(const Params& p, int64_t tok0, int nt, float2* cs) {
 
 // How a lane holds its V elements of a row, and which of them are pairs.
 enum Mode : int {
-  kHalves = 0,  // V/2 elements from each half of the row: pairs (j, j + V/2); the whole row is rotated
+  kHalves = 0,  // V/2 elements from each half of the rotated part: pairs (j, j + V/2); behind it V in a row
   kRun = 1,     // V elements in a row: pairs (2j, 2j + 1), those behind `rotary` turn by 0
 };
 
@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
   __syncthreads();
   // column of element j of this lane's vector i
   auto col = [&](int i, int j) {
-    return MODE == kHalves ? (i * G + gl) * H + (j < H ? j : j - H + p.dim / 2) : (i * G + gl) * V + j;
+    const int v = i * G + gl;
+    return MODE == kHalves && v * V < p.rotary ? v * H + (j < H ? j : j - H + half) : v * V + j;
   };
   const bool has[2] = {gl * V < p.dim, NV > 1 && (G + gl) * V < p.dim};  // dim is a multiple of V
   float dw[2][NV][V];
@@ -94,8 +95,8 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
   }
   auto load = [&](const T* row, int i) {
     if (MODE == kRun) return *reinterpret_cast<const uint4*>(row + (i * G + gl) * V);
-    const uint2 a = *reinterpret_cast<const uint2*>(row + (i * G + gl) * H);
-    const uint2 b = *reinterpret_cast<const uint2*>(row + p.dim / 2 + (i * G + gl) * H);
+    const uint2 a = *reinterpret_cast<const uint2*>(row + col(i, 0));
+    const uint2 b = *reinterpret_cast<const uint2*>(row + col(i, H));
     return make_uint4(a.x, a.y, b.x, b.y);
   };
   auto store = [&](T* row, int i, const float (&v)[V]) {
@@ -106,8 +107,8 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
     if (MODE == kRun) {
       *reinterpret_cast<uint4*>(row + (i * G + gl) * V) = raw;
     } else {
-      *reinterpret_cast<uint2*>(row + (i * G + gl) * H) = make_uint2(raw.x, raw.y);
-      *reinterpret_cast<uint2*>(row + p.dim / 2 + (i * G + gl) * H) = make_uint2(raw.z, raw.w);
+      *reinterpret_cast<uint2*>(row + col(i, 0)) = make_uint2(raw.x, raw.y);
+      *reinterpret_cast<uint2*>(row + col(i, H)) = make_uint2(raw.z, raw.w);
     }
   };
   for (int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block; tok0 < tokens; tok0 += (int64_t)gridDim.x * p.tokens_per_block) {
@@ -368,8 +369,8 @@ static hxm_status launch_vec(Params& p, cudaStream_t st) {
 template <typename T, bool BWD>
 static hxm_status launch(Params& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  // the register kernel: whole vectors, and halves that are rotated entirely or not at all
-  bool vec = p.dim % V == 0 && p.dim <= 64 * V && (p.interleaved || p.rotary == 0 || p.rotary == p.dim);
+  // the register kernel: whole vectors, in the rotated part too where its pairs lie half of it apart
+  bool vec = p.dim % V == 0 && p.dim <= 64 * V && (p.interleaved || p.rotary % V == 0);
   for (int i = 0; i < 2; ++i) {
     const Side& s = p.s[i];
     auto ok = [&](const void* ptr, const int64_t* st3) {
