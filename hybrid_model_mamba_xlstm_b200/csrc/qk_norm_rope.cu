@@ -4,6 +4,8 @@
 // Replaces the two per-head norms of mLSTMBlock.forward (hybrid_xmamba/layers/mlstm_block.py:113-114,
 // RMSNorm.forward of layers/normalization.py:32-34) for layers that also rotate q and k.  HBM-bound:
 // x is read once and y written once (gradients: x and dy read, dx written).
+// 8 x 2048 tokens of 16 + 4 heads of 128, bf16: 33.5 us, 5.0 TB/s; gradients 62 us, 4.0 TB/s (latency: two blocks
+// of 256 threads fit an SM).
 //
 // A row is one head of one token.  With n = x / sqrt(mean x^2 + eps) and y = R (w * n), R turning the
 // pairs, the gradients are g = R^T dy, dw = sum over rows of g * n, and
@@ -38,7 +40,7 @@ struct Params {
   double log2_base;
   float eps;
   float* partial;  // gradients: (blocks, 2, dim) weight sums
-  int tokens_per_block;
+  int tokens_per_block, blocks;
 };
 
 // cos, sin of every pair of `nt` tokens from token `tok0` on, into cs[token * rotary/2 + pair].
@@ -62,12 +64,33 @@ enum Mode : int {
   kRun = 1,     // V elements in a row: pairs (2j, 2j + 1), those behind `rotary` turn by 0
 };
 
+// 16 bytes of a row as float2s, and back (the one rounding of a 16-bit result).
+template <typename T>
+HXM_DEV void widen(const uint4& raw, float2 (&v)[8 / sizeof(T)]) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int j = 0; j < (int)(8 / sizeof(T)); ++j) v[j] = make_float2(to_f32<T>(e[2 * j]), to_f32<T>(e[2 * j + 1]));
+}
+template <typename T>
+HXM_DEV uint4 narrow(const float2 (&v)[8 / sizeof(T)]) {
+  uint4 raw;
+  T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+  for (int j = 0; j < (int)(8 / sizeof(T)); ++j) {
+    e[2 * j] = from_f32<T>(v[j].x);
+    e[2 * j + 1] = from_f32<T>(v[j].y);
+  }
+  return raw;
+}
+HXM_DEV float2 both(float a) { return make_float2(a, a); }
+
 // Rows that fit the registers of G <= 32 lanes, NV * 16 bytes a lane.  A group of G lanes takes one token
 // and every (256 / G / tokens_per_block)-th of its heads, so a lane's cosines and sines serve all of its
-// rows; R rows are loaded before the first is worked on, for the latency of HBM.
+// rows; R rows are loaded before the first is worked on, for the latency of HBM.  The instructions weigh as
+// much as the bytes (some 100 a row and lane), so the arithmetic goes two elements at a time.
 template <typename T, int G, int NV, int MODE, bool BWD>
 __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
-  constexpr int V = 16 / sizeof(T), H = V / 2, R = NV > 1 ? 2 : (BWD ? 2 : 4);
+  constexpr int V = 16 / sizeof(T), H = V / 2, F = V / 2, A = V / 4, R = NV > 1 ? 2 : 4;
   extern __shared__ __align__(16) unsigned char shraw[];
   double* freq = reinterpret_cast<double*>(shraw);  // turns per position of each pair
   const int half = p.rotary / 2;
@@ -84,14 +107,14 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
     return MODE == kHalves && v * V < p.rotary ? v * H + (j < H ? j : j - H + half) : v * V + j;
   };
   const bool has[2] = {gl * V < p.dim, NV > 1 && (G + gl) * V < p.dim};  // dim is a multiple of V
-  float dw[2][NV][V];
+  float2 dw[2][NV][F];
   if (BWD) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) dw[s][i][j] = 0.f;
+        for (int j = 0; j < F; ++j) dw[s][i][j] = both(0.f);
   }
   auto load = [&](const T* row, int i) {
     if (MODE == kRun) return *reinterpret_cast<const uint4*>(row + (i * G + gl) * V);
@@ -99,11 +122,7 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
     const uint2 b = *reinterpret_cast<const uint2*>(row + col(i, H));
     return make_uint4(a.x, a.y, b.x, b.y);
   };
-  auto store = [&](T* row, int i, const float (&v)[V]) {
-    uint4 raw;
-    T* e = reinterpret_cast<T*>(&raw);
-#pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = from_f32<T>(v[j]);
+  auto store = [&](T* row, int i, const uint4& raw) {
     if (MODE == kRun) {
       *reinterpret_cast<uint4*>(row + (i * G + gl) * V) = raw;
     } else {
@@ -111,11 +130,12 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
       *reinterpret_cast<uint2*>(row + col(i, H)) = make_uint2(raw.z, raw.w);
     }
   };
+  const float per_dim = 1.f / (float)p.dim;
   for (int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block; tok0 < tokens; tok0 += (int64_t)gridDim.x * p.tokens_per_block) {
     const int64_t tok = tok0 + it;
     const bool here = tok < tokens;
     const int64_t b = here ? tok / p.seqlen : 0, t = here ? tok - b * p.seqlen : 0;
-    float2 cs[NV][H];
+    float2 cs[NV][A], sn[NV][A];  // of pairs 2j, 2j + 1 of this lane; the gradients turn back
     if (half) {
       const int64_t at = here ? p.pos[b * p.spos[0] + t * p.spos[1]] : 0;
 #pragma unroll
@@ -124,96 +144,107 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
         for (int j = 0; j < H; ++j) {
           const int pr = (i * G + gl) * H + j;
           const double turns = (double)at * freq[pr < half ? pr : 0];
-          float sn, c;
-          sincospif((float)(2.0 * (turns - rint(turns))), &sn, &c);
-          cs[i][j] = pr < half ? make_float2(c, sn) : make_float2(1.f, 0.f);
+          float s, c;
+          sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+          if (pr >= half) c = 1.f, s = 0.f;
+          if (BWD) s = -s;
+          (j & 1 ? cs[i][j / 2].y : cs[i][j / 2].x) = c;
+          (j & 1 ? sn[i][j / 2].y : sn[i][j / 2].x) = s;
         }
     }
-    auto turn = [&](float (&y)[V], int i, float sign) {
+    auto turn = [&](float2 (&y)[F], int i) {
       if (!half) return;
+      if (MODE == kHalves) {
 #pragma unroll
-      for (int j = 0; j < H; ++j) {
-        float &u = y[MODE == kHalves ? j : 2 * j], &v = y[MODE == kHalves ? j + H : 2 * j + 1];
-        const float c = cs[i][j].x, sn = sign * cs[i][j].y, a = u;
-        u = a * c - v * sn;
-        v = v * c + a * sn;
+        for (int j = 0; j < A; ++j) {
+          const float2 u = y[j], v = y[A + j], c = cs[i][j], s = sn[i][j];
+          y[j] = __ffma2_rn(u, c, __fmul2_rn(make_float2(-v.x, -v.y), s));
+          y[A + j] = __ffma2_rn(v, c, __fmul2_rn(u, s));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+          const float c = j & 1 ? cs[i][j / 2].y : cs[i][j / 2].x, s = j & 1 ? sn[i][j / 2].y : sn[i][j / 2].x;
+          const float2 u = y[j];
+          y[j] = make_float2(u.x * c - u.y * s, u.y * c + u.x * s);
+        }
       }
     };
 #pragma unroll
     for (int sd = 0; sd < 2; ++sd) {
       const Side& s = p.s[sd];
-      float w[NV][V];
+      float2 w[NV][F];
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) w[i][j] = s.w && has[i] ? s.w[col(i, j)] : 1.f;
-      const T* xt = static_cast<const T*>(s.x) + b * s.sx[0] + t * s.sx[1];
-      const T* gt = BWD ? static_cast<const T*>(s.g) + b * s.sg[0] + t * s.sg[1] : nullptr;
-      T* ot = static_cast<T*>(s.out) + b * s.so[0] + t * s.so[1];
+        for (int j = 0; j < F; ++j) w[i][j] = s.w && has[i] ? *reinterpret_cast<const float2*>(s.w + col(i, 2 * j)) : both(1.f);
+      const T* xt = static_cast<const T*>(s.x) + b * s.sx[0] + t * s.sx[1] + h0 * s.sx[2];
+      const T* gt = BWD ? static_cast<const T*>(s.g) + b * s.sg[0] + t * s.sg[1] + h0 * s.sg[2] : nullptr;
+      T* ot = static_cast<T*>(s.out) + b * s.so[0] + t * s.so[1] + h0 * s.so[2];
+      const int64_t xs = hs * s.sx[2], gs = BWD ? hs * s.sg[2] : 0, os = hs * s.so[2];
+      const int rows = here ? s.heads - h0 : 0;  // of this lane: those r with r * hs < rows
       // every lane of the warp goes through the loop (the shuffles need them all)
       for (int hb = 0; hb < s.heads; hb += R * hs) {
         uint4 xr[R][NV], gr[R][NV];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int h = hb + r * hs + h0;
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            const bool live = here && h < s.heads && has[i];
-            xr[r][i] = live ? load(xt + h * s.sx[2], i) : make_uint4(0, 0, 0, 0);
-            if (BWD) gr[r][i] = live ? load(gt + h * s.sg[2], i) : make_uint4(0, 0, 0, 0);
+            const bool live = hb + r * hs < rows && has[i];
+            xr[r][i] = live ? load(xt, i) : make_uint4(0, 0, 0, 0);
+            if (BWD) gr[r][i] = live ? load(gt, i) : make_uint4(0, 0, 0, 0);
           }
+          xt += xs;
+          if (BWD) gt += gs;
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const int h = hb + r * hs + h0;
           if (hb + r * hs >= s.heads) break;  // block-uniform
-          float x[NV][V], ssq = 0.f;
+          float2 x[NV][F], sq = both(0.f);
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            const T* e = reinterpret_cast<const T*>(&xr[r][i]);
+            widen<T>(xr[r][i], x[i]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              x[i][j] = to_f32<T>(e[j]);
-              ssq = fmaf(x[i][j], x[i][j], ssq);
-            }
+            for (int j = 0; j < F; ++j) sq = __ffma2_rn(x[i][j], x[i][j], sq);
           }
+          float ssq = sq.x + sq.y;
 #pragma unroll
           for (int o = G / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-          const float inv = rsqrtf(ssq / (float)p.dim + p.eps);
+          const float2 inv = both(rsqrtf(fmaf(ssq, per_dim, p.eps)));
           if (!BWD) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
 #pragma unroll
-              for (int j = 0; j < V; ++j) x[i][j] = x[i][j] * inv * w[i][j];
-              turn(x[i], i, 1.f);
+              for (int j = 0; j < F; ++j) x[i][j] = __fmul2_rn(__fmul2_rn(x[i][j], inv), w[i][j]);
+              turn(x[i], i);
             }
           } else {
-            float g[NV][V], m = 0.f;
+            float2 g[NV][F], mm = both(0.f);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-              const T* e = reinterpret_cast<const T*>(&gr[r][i]);
+              widen<T>(gr[r][i], g[i]);
+              turn(g[i], i);
 #pragma unroll
-              for (int j = 0; j < V; ++j) g[i][j] = to_f32<T>(e[j]);
-              turn(g[i], i, -1.f);
-#pragma unroll
-              for (int j = 0; j < V; ++j) {
-                x[i][j] *= inv;
-                const float gn = g[i][j] * x[i][j];
-                dw[sd][i][j] += gn;  // 0 where this lane has no row
-                m = fmaf(gn, w[i][j], m);
+              for (int j = 0; j < F; ++j) {
+                x[i][j] = __fmul2_rn(x[i][j], inv);
+                const float2 gn = __fmul2_rn(g[i][j], x[i][j]);
+                dw[sd][i][j] = __fadd2_rn(dw[sd][i][j], gn);  // 0 where this lane has no row
+                mm = __ffma2_rn(gn, w[i][j], mm);
               }
             }
+            float m = mm.x + mm.y;
 #pragma unroll
             for (int o = G / 2; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-            m /= (float)p.dim;
+            const float2 mean = both(-m * per_dim);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-              for (int j = 0; j < V; ++j) x[i][j] = inv * (w[i][j] * g[i][j] - x[i][j] * m);
+              for (int j = 0; j < F; ++j) x[i][j] = __fmul2_rn(inv, __ffma2_rn(x[i][j], mean, __fmul2_rn(w[i][j], g[i][j])));
           }
 #pragma unroll
           for (int i = 0; i < NV; ++i)
-            if (here && h < s.heads && has[i]) store(ot + h * s.so[2], i, x[i]);
+            if (hb + r * hs < rows && has[i]) store(ot, i, narrow<T>(x[i]));
+          ot += os;
         }
       }
     }
@@ -227,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
       for (int i = 0; i < NV; ++i)
         if (has[i])
 #pragma unroll
-          for (int j = 0; j < V; ++j) red[group * p.dim + col(i, j)] = dw[sd][i][j];
+          for (int j = 0; j < F; ++j) *reinterpret_cast<float2*>(red + group * p.dim + col(i, 2 * j)) = dw[sd][i][j];
       __syncthreads();
       for (int c = threadIdx.x; c < p.dim; c += kThreads) {
         float a = 0.f;
@@ -337,16 +368,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const float* partial, in
 }
 
 constexpr int kSMs = 148;
-// Blocks whose weight sums the gradients keep: four per SM.
-constexpr int kBwdBlocks = 4 * kSMs;
+// Blocks whose weight sums the gradients keep: the two per SM that are resident (with four, in two waves,
+// 8 x 2048 x 20 x 128 took 75 us instead of 62), of the shared-memory kernel four (604 us with two, 357).
+constexpr int kBwdBlocks = 2 * kSMs, kBwdBlocksRow = 4 * kSMs;
 
 template <typename T, int G, int NV, int MODE, bool BWD>
 static hxm_status launch_mode(Params& p, cudaStream_t st) {
   const int64_t tokens = (int64_t)p.batch * p.seqlen;
-  // tokens a block takes at once: one while blocks are few, for their number; up to 8 (every group keeps
-  // some heads), so that a lane's angles serve more rows
+  // tokens a block takes at once: one while blocks are few, for their number; up to 16, so that a lane's
+  // angles serve more rows (8 x 2048 x 20 x 128 bf16 33.5 us, with up to 8 36.5); gradients 8, whose blocks
+  // then have even shares
   int tpb = 1;
-  while (tpb < 8 && tpb * 2 <= kThreads / G && tokens / (tpb * 2) >= 4 * kSMs) tpb *= 2;
+  while (tpb < (BWD ? 8 : 16) && tpb * 2 <= kThreads / G && tokens / (tpb * 2) >= 4 * kSMs) tpb *= 2;
   p.tokens_per_block = tpb;
   int64_t grid = (tokens + tpb - 1) / tpb;
   if (grid > 16 * kSMs) grid = 16 * kSMs;  // the pairs' frequencies are made once a block
@@ -354,8 +387,8 @@ static hxm_status launch_mode(Params& p, cudaStream_t st) {
   if (BWD) {
     const size_t red = (size_t)(kThreads / G) * p.dim * sizeof(float);
     if (red > smem) smem = red;
-    // blocks that take no token write zeros: the join always reads kBwdBlocks sums
-    grid = kBwdBlocks;
+    // blocks that take no token write zeros: the join reads all sums
+    grid = p.blocks = kBwdBlocks;
   }
   vec_kernel<T, G, NV, MODE, BWD><<<(unsigned)grid, kThreads, smem, st>>>(p);
   return check_launch("hxm_qk_norm_rope");
@@ -376,7 +409,7 @@ static hxm_status launch(Params& p, cudaStream_t st) {
     auto ok = [&](const void* ptr, const int64_t* st3) {
       return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && st3[0] % V == 0 && st3[1] % V == 0 && st3[2] % V == 0;
     };
-    vec = vec && (s.heads == 0 || (ok(s.x, s.sx) && ok(s.out, s.so) && (!BWD || ok(s.g, s.sg))));
+    vec = vec && reinterpret_cast<uintptr_t>(s.w) % 8 == 0 && (s.heads == 0 || (ok(s.x, s.sx) && ok(s.out, s.so) && (!BWD || ok(s.g, s.sg))));
   }
   if (vec) {
     const int nvec = p.dim / V;
@@ -387,7 +420,7 @@ static hxm_status launch(Params& p, cudaStream_t st) {
     return launch_vec<T, 32, 2, BWD>(p, st);
   }
   const int64_t tokens = (int64_t)p.batch * p.seqlen;
-  const unsigned grid = BWD ? kBwdBlocks : (unsigned)(tokens < 16 * kSMs ? tokens : 16 * kSMs);
+  const unsigned grid = BWD ? (unsigned)(p.blocks = kBwdBlocksRow) : (unsigned)(tokens < 16 * kSMs ? tokens : 16 * kSMs);
   const size_t smem = (size_t)(p.rotary / 2) * sizeof(float2) + sizeof(float) * p.dim * (kThreads / 32) * (BWD ? 4 : 2);
   HXM_CUDA_TRY(cudaFuncSetAttribute(row_kernel<T, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   row_kernel<T, BWD><<<grid, kThreads, smem, st>>>(p);
@@ -452,7 +485,7 @@ static hxm_status check_bwd(const hxm_qk_norm_rope_bwd_args* a, const char* who)
 
 extern "C" size_t hxm_qk_norm_rope_bwd_workspace_size(const hxm_qk_norm_rope_bwd_args* a) {
   if (check_bwd(a, "hxm_qk_norm_rope_bwd_workspace_size") != HXM_OK) return 0;
-  return sizeof(float) * 2 * (size_t)a->fwd.dim * kBwdBlocks;
+  return sizeof(float) * 2 * (size_t)a->fwd.dim * kBwdBlocksRow;
 }
 
 extern "C" hxm_status hxm_qk_norm_rope_bwd(const hxm_qk_norm_rope_bwd_args* a, void* stream) {
@@ -468,7 +501,7 @@ extern "C" hxm_status hxm_qk_norm_rope_bwd(const hxm_qk_norm_rope_bwd_args* a, v
   }
   HXM_REQUIRE((f.heads_q == 0 || (f.q && f.q_out && a->dq_out)) && (f.heads_k == 0 || (f.k && f.k_out && a->dk_out)) &&
                   (f.rotary == 0 || f.positions), "hxm_qk_norm_rope_bwd: NULL tensor pointer");
-  const size_t need = sizeof(float) * 2 * (size_t)f.dim * kBwdBlocks;
+  const size_t need = sizeof(float) * 2 * (size_t)f.dim * kBwdBlocksRow;
   HXM_REQUIRE(a->workspace && a->workspace_bytes >= need, "hxm_qk_norm_rope_bwd: workspace %zu bytes < %zu", a->workspace_bytes, need);
   Params p = make_params(&f);
   p.s[0].g = a->dq_out; p.s[1].g = a->dk_out;
@@ -477,6 +510,6 @@ extern "C" hxm_status hxm_qk_norm_rope_bwd(const hxm_qk_norm_rope_bwd_args* a, v
   const hxm_status r = f.io_dtype == HXM_F32 ? launch<float, true>(p, st)
                        : f.io_dtype == HXM_BF16 ? launch<__nv_bfloat16, true>(p, st) : launch<__half, true>(p, st);
   if (r != HXM_OK || (!a->dq_weight && !a->dk_weight)) return r;
-  join_kernel<<<(2 * f.dim + 31) / 32, kThreads, 0, st>>>(p.partial, kBwdBlocks, f.dim, a->dq_weight, a->dk_weight);
+  join_kernel<<<(2 * f.dim + 31) / 32, kThreads, 0, st>>>(p.partial, p.blocks, f.dim, a->dq_weight, a->dk_weight);
   return check_launch("hxm_qk_norm_rope_bwd");
 }
