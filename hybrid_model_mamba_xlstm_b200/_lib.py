@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as ct
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -416,6 +417,23 @@ def lib() -> ct.CDLL:
                     f.argtypes = args
                 _lib = l
     return _lib
+
+
+def packer(cls):
+    """f(*values) -> cls, from the values of its fields in order, arrays element by element, a nested struct as one
+    (NULL is 0): a quarter of the time that setting some forty values by name takes."""
+    code = {ct.c_int32: "i", ct.c_int64: "q", ct.c_size_t: "N", ct.c_void_p: "P", ct.c_float: "f", ct.c_double: "d"}
+    parts = []
+    for _, t in cls._fields_:
+        if issubclass(t, ct.Structure):
+            parts.append(f"{ct.sizeof(t)}s")
+        elif issubclass(t, ct.Array):
+            parts.append(f"{t._length_}{code[t._type_]}")
+        else:
+            parts.append(code[t])
+    layout = struct.Struct("@" + "".join(parts) + "0P")
+    assert layout.size == ct.sizeof(cls)
+    return lambda *values: cls.from_buffer_copy(layout.pack(*values))
 
 
 def check(fn: str, status: int):

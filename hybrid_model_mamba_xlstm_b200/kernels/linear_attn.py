@@ -13,9 +13,13 @@ import math
 import torch
 
 from .. import _lib
-from ._common import dtype_code, on_device, once_only, ptr, require_cuda, stream_of
+from ._common import dtype_code, on_device, once_only, require_cuda, stream_of
 
 __all__ = ["linear_attention", "linear_attention_bwd", "linear_attention_step"]
+
+_fwd_args, _bwd_args, _step_args = (_lib.packer(c) for c in (_lib.LinearAttnArgs, _lib.LinearAttnBwdArgs, _lib.LinearAttnStepArgs))
+_FWD, _BWD, _STEP = (ctypes.sizeof(c) for c in (_lib.LinearAttnArgs, _lib.LinearAttnBwdArgs, _lib.LinearAttnStepArgs))
+_NONE = (0,) * 5  # an absent state: address and strides
 
 
 def _check_io(who, q, k, v):
@@ -23,6 +27,14 @@ def _check_io(who, q, k, v):
         raise TypeError(f"{who}: q must be fp32 or bf16, got {q.dtype}")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"{who}: q, k, v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+
+
+def _check(who, q, k, v):
+    if q.dim() != 4:
+        raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
+    if k.shape != q.shape or v.shape[:-1] != q.shape[:-1] or v.dim() != 4:
+        raise ValueError(f"{who}: k must be {tuple(q.shape)} and v (B, L, H, dv), got {tuple(k.shape)}, {tuple(v.shape)}")
+    _check_io(who, q, k, v)
 
 
 def _scale(who, scale, dk):
@@ -46,24 +58,22 @@ def _rows(t):
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         return t.contiguous()
     e = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and t.is_contiguous():
+        return t
     if t.shape[-1] % e == 0 and (t.data_ptr() % 16 or any(s % e for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
         return t.contiguous() if not t.is_contiguous() else t.clone()
     return t
 
 
-def _set(a, name, t, n):
-    setattr(a, name, t.data_ptr())
-    setattr(a, name + "_stride", tuple(s if m > 1 else 0 for s, m in zip(t.stride()[:n], t.shape[:n])))
+def _at(t):
+    """Address and strides of t (B, L, H, d); those of extents of 1 count for nothing and are 0."""
+    s, n = t.stride(), t.shape
+    return t.data_ptr(), s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0
 
 
-def _fill(who, q, k, v, log_decay, scale, lengths, s0, error_flag, wait_limit_cycles):
-    """(args, tensors to keep alive) of the fields that the forward and the backward share."""
-    if q.dim() != 4:
-        raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
+def _fill(who, q, k, v, log_decay, scale, lengths, s0, out, sT, error_flag, wait_limit_cycles):
+    """(args of the forward, tensors to keep alive); out and sT: where the backward has none, None."""
     bsz, L, nh, dk = q.shape
-    if k.shape != q.shape or v.shape[:-1] != q.shape[:-1] or v.dim() != 4:
-        raise ValueError(f"{who}: k must be {tuple(q.shape)} and v (B, L, H, dv), got {tuple(k.shape)}, {tuple(v.shape)}")
-    _check_io(who, q, k, v)
     if lengths is not None:
         if lengths.shape != (bsz,) or lengths.is_floating_point() or lengths.dtype == torch.bool:
             raise ValueError(f"{who}: lengths must be ({bsz},) integers")
@@ -76,18 +86,11 @@ def _fill(who, q, k, v, log_decay, scale, lengths, s0, error_flag, wait_limit_cy
         s0 = s0.float()
     q, k, v = _rows(q), _rows(k), _rows(v)
     ld = _decay(who, log_decay, nh)
-    a = _lib.LinearAttnArgs()
-    a.struct_size = ctypes.sizeof(a)
-    a.batch, a.seqlen, a.heads, a.dk, a.dv = bsz, L, nh, dk, v.shape[-1]
-    a.io_dtype = dtype_code(q)
-    _set(a, "q", q, 3)
-    _set(a, "k", k, 3)
-    _set(a, "v", v, 3)
-    a.log_decay, a.lengths = ptr(ld), ptr(lengths)
-    if s0 is not None:
-        a.s0, a.s0_stride = s0.data_ptr(), s0.stride()
-    a.scale = scale
-    a.error_flag, a.wait_limit_cycles = ptr(error_flag), int(wait_limit_cycles)
+    a = _fwd_args(_FWD, bsz, L, nh, dk, v.shape[-1], dtype_code(q), *_at(q), *_at(k), *_at(v),
+                  *(_NONE[:4] if out is None else _at(out)), ld.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                  *(_NONE if s0 is None else (s0.data_ptr(), *s0.stride())),
+                  *(_NONE if sT is None else (sT.data_ptr(), *sT.stride())),
+                  scale, 0, 0, 0 if error_flag is None else error_flag.data_ptr(), int(wait_limit_cycles))
     return a, (q, k, v, ld, lengths, s0)
 
 
@@ -95,16 +98,14 @@ def _forward(q, k, v, log_decay, scale, lengths, s0, want_state, error_flag=None
     who = "linear_attention"
     dev = require_cuda(q, k, v, log_decay, lengths, s0, error_flag, who=who)
     with on_device(dev):
-        a, keep = _fill(who, q, k, v, log_decay, scale, lengths, s0, error_flag, wait_limit_cycles)
-        out = torch.empty(a.batch, a.seqlen, a.heads, a.dv, device=dev, dtype=q.dtype)
-        _set(a, "out", out, 3)
-        sT = None
-        if want_state:
-            sT = torch.empty(a.batch, a.heads, a.dk, a.dv, device=dev, dtype=torch.float32)
-            a.sT, a.sT_stride = sT.data_ptr(), sT.stride()
-        n = int(_lib.lib().hxm_linear_attn_workspace_size(a))
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-        a.workspace, a.workspace_bytes = ptr(ws), n
+        _check(who, q, k, v)
+        out = torch.empty(v.shape, device=dev, dtype=q.dtype)
+        sT = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], device=dev, dtype=torch.float32) if want_state else None
+        a, keep = _fill(who, q, k, v, log_decay, scale, lengths, s0, out, sT, error_flag, wait_limit_cycles)
+        n = _lib.lib().hxm_linear_attn_workspace_size(a)
+        if n:
+            ws = torch.empty(n, device=dev, dtype=torch.uint8)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
         _lib.call("hxm_linear_attn_fwd", a, stream_of(dev))
     return out, sT
 
@@ -124,26 +125,25 @@ def linear_attention_bwd(q, k, v, log_decay, dout, *, scale=None, lengths=None, 
     if need_d_initial_state is None:
         need_d_initial_state = initial_state is not None
     with on_device(dev):
-        f, keep = _fill(who, q, k, v, log_decay, scale, lengths, initial_state, error_flag, wait_limit_cycles)
+        _check(who, q, k, v)
+        f, keep = _fill(who, q, k, v, log_decay, scale, lengths, initial_state, None, None, error_flag, wait_limit_cycles)
         dout = _rows(dout)
-        a = _lib.LinearAttnBwdArgs()
-        a.fwd = f
-        a.struct_size = ctypes.sizeof(a)
-        _set(a, "dout", dout, 3)
-        sshape = (f.batch, f.heads, f.dk, f.dv)
+        sshape = (q.shape[0], q.shape[2], q.shape[3], v.shape[3])
         if d_final_state is not None:
             if d_final_state.shape != sshape:
                 raise ValueError(f"{who}: d_final_state must be {sshape}, got {tuple(d_final_state.shape)}")
             d_final_state = d_final_state.float()
-            a.dsT, a.dsT_stride = d_final_state.data_ptr(), d_final_state.stride()
         dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
         dk = torch.empty(q.shape, device=dev, dtype=q.dtype)
         dv = torch.empty(v.shape, device=dev, dtype=q.dtype)
         ds0 = torch.empty(sshape, device=dev, dtype=torch.float32) if need_d_initial_state else None
-        a.dq, a.dk, a.dv, a.ds0 = ptr(dq), ptr(dk), ptr(dv), ptr(ds0)
-        n = int(_lib.lib().hxm_linear_attn_bwd_workspace_size(a))
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-        a.workspace, a.workspace_bytes = ptr(ws), n
+        a = _bwd_args(bytes(f), _BWD, *_at(dout),
+                      *(_NONE if d_final_state is None else (d_final_state.data_ptr(), *d_final_state.stride())),
+                      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), 0 if ds0 is None else ds0.data_ptr(), 0, 0)
+        n = _lib.lib().hxm_linear_attn_bwd_workspace_size(a)
+        if n:
+            ws = torch.empty(n, device=dev, dtype=torch.uint8)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
         _lib.call("hxm_linear_attn_bwd", a, stream_of(dev))
     return dq, dk, dv, ds0
 
@@ -234,12 +234,8 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
         elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1) or any(
                 s == 0 for s, n in zip(out.stride(), out.shape) if n > 1):
             raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride and no repeated rows")
-        a = _lib.LinearAttnStepArgs()
-        a.batch, a.heads, a.dk, a.dv = bsz, nh, dk, dv
-        a.io_dtype = dtype_code(q)
-        for name, t, n in (("q", q, 2), ("k", k, 2), ("v", v, 2), ("out", out, 2), ("state", state, 3)):
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_stride", t.stride()[:n])
-        a.log_decay, a.scale = ptr(ld), scale
+        a = _step_args(_STEP, bsz, nh, dk, dv, dtype_code(q), q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
+                       v.data_ptr(), *v.stride()[:2], out.data_ptr(), *out.stride()[:2], ld.data_ptr(), state.data_ptr(),
+                       *state.stride()[:3], scale)
         _lib.call("hxm_linear_attn_step", a, stream_of(dev))
     return out

@@ -15,12 +15,16 @@ from ._common import dtype_code, f32_param, on_device, once_only, ptr, require_c
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_bwd"]
 
+_fwd_args, _bwd_args = _lib.packer(_lib.QkNormRopeArgs), _lib.packer(_lib.QkNormRopeBwdArgs)
+_FWD, _BWD = ctypes.sizeof(_lib.QkNormRopeArgs), ctypes.sizeof(_lib.QkNormRopeBwdArgs)
+
 
 def _unit(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
+    """(args of the forward with new dense outputs, these, tensors to keep alive)."""
     if q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[-1] != q.shape[-1]:
         raise ValueError(f"{who}: q must be (B, L, Hq, d) and k (B, L, Hk, d), got {tuple(q.shape)}, {tuple(k.shape)}")
     if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or k.dtype != q.dtype:
@@ -38,33 +42,26 @@ def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
         raise ValueError(f"{who}: rope_base must be positive and finite, got {base}")
     q, k = _unit(q), _unit(k)
     qw, kw = f32_param(qw), f32_param(kw)
-    a = _lib.QkNormRopeArgs()
-    a.struct_size = ctypes.sizeof(a)
-    a.batch, a.seqlen, a.heads_q, a.heads_k, a.dim, a.rotary = bsz, L, hq, k.shape[2], d, rotary
-    a.io_dtype, a.interleaved = dtype_code(q), int(bool(interleaved))
-    a.q, a.q_stride = q.data_ptr(), q.stride()[:3]
-    a.k, a.k_stride = k.data_ptr(), k.stride()[:3]
-    a.q_weight, a.k_weight = ptr(qw), ptr(kw)
+    at = (0, 0, 0)
     if rotary:
         if positions.is_floating_point() or positions.dtype == torch.bool or positions.shape not in ((bsz, L), (L,)):
             raise ValueError(f"{who}: positions must be integers ({bsz}, {L}) or ({L},), got {positions.dtype} "
                              f"{tuple(positions.shape)}")
         positions = positions.long()
-        a.positions = positions.data_ptr()
-        a.positions_stride = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    a.rope_base, a.eps = float(base), float(eps)
-    return a, (q, k, qw, kw, positions)
+        at = (positions.data_ptr(), *(positions.stride() if positions.dim() == 2 else (0, positions.stride(0))))
+    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    yk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    a = _fwd_args(_FWD, bsz, L, hq, k.shape[2], d, rotary, dtype_code(q), bool(interleaved),
+                  q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], ptr(qw) or 0, ptr(kw) or 0, *at,
+                  float(base), float(eps), yq.data_ptr(), *yq.stride()[:3], yk.data_ptr(), *yk.stride()[:3])
+    return a, yq, yk, (q, k, qw, kw, positions)
 
 
 def _forward(q, k, qw, kw, positions, base, rotary, interleaved, eps):
     who = "qk_norm_rope"
     dev = require_cuda(q, k, qw, kw, positions, who=who)
     with on_device(dev):
-        a, keep = _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps)
-        yq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        yk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        a.q_out, a.q_out_stride = yq.data_ptr(), yq.stride()[:3]
-        a.k_out, a.k_out_stride = yk.data_ptr(), yk.stride()[:3]
+        a, yq, yk, keep = _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps)
         _lib.call("hxm_qk_norm_rope_fwd", a, stream_of(dev))
     return yq, yk
 
@@ -79,22 +76,14 @@ def qk_norm_rope_bwd(q, k, q_weight, k_weight, dq_out, dk_out, positions=None, *
     if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.dtype != q.dtype or dk_out.dtype != k.dtype:
         raise ValueError(f"{who}: the gradients must match q and k")
     with on_device(dev):
-        f, keep = _fill(who, q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=dev, dtype=k.dtype)
-        f.q_out, f.q_out_stride = dq.data_ptr(), dq.stride()[:3]
-        f.k_out, f.k_out_stride = dk.data_ptr(), dk.stride()[:3]
+        f, dq, dk, keep = _fill(who, q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)
         dq_out, dk_out = _unit(dq_out), _unit(dk_out)
-        a = _lib.QkNormRopeBwdArgs()
-        a.fwd = f
-        a.struct_size = ctypes.sizeof(a)
-        a.dq_out, a.dq_out_stride = dq_out.data_ptr(), dq_out.stride()[:3]
-        a.dk_out, a.dk_out_stride = dk_out.data_ptr(), dk_out.stride()[:3]
         d = q.shape[-1]
         dw = [torch.empty(d, device=dev, dtype=torch.float32) if weight_grads and w is not None else None
               for w in (q_weight, k_weight)]
-        a.dq_weight, a.dk_weight = ptr(dw[0]), ptr(dw[1])
-        n = int(_lib.lib().hxm_qk_norm_rope_bwd_workspace_size(a))
+        a = _bwd_args(bytes(f), _BWD, dq_out.data_ptr(), *dq_out.stride()[:3], dk_out.data_ptr(), *dk_out.stride()[:3],
+                      ptr(dw[0]) or 0, ptr(dw[1]) or 0, 0, 0)
+        n = _lib.lib().hxm_qk_norm_rope_bwd_workspace_size(a)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ptr(ws), n
         _lib.call("hxm_qk_norm_rope_bwd", a, stream_of(dev))
