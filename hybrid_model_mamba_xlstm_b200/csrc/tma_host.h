@@ -37,9 +37,20 @@ inline hxm_status make_map_bf16_4d(CUtensorMap* map, const void* base, const uin
   cuuint64_t st[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
   cuuint32_t box[4] = {64, box_rows, 1, 1};
   cuuint32_t es[4] = {1, 1, 1, 1};
-  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, box, es,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto make = [&] {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, box, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = make();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A driver call needs a context bound to the calling thread, which a thread has only from its first
+    // runtime call on (a thread of the caller's, or autograd's: its memory may come from a cache).
+    int dev = 0;
+    HXM_CUDA_TRY(cudaGetDevice(&dev));
+    HXM_CUDA_TRY(cudaSetDevice(dev));
+    r = make();
+  }
   if (r != CUDA_SUCCESS) {
     set_error("%s: cuTensorMapEncodeTiled failed (%d)", who, (int)r);
     return HXM_ECUDA;

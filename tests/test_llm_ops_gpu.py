@@ -5,7 +5,7 @@ Tolerance of the fp32 runs: an element of q or k comes from a sum of d squares a
 attention from at most L + dk + dv terms, each with a relative error of 2^-24: (L + dk + dv + 2 d + 64) 2^-24 times
 the same sum over absolute values (two norms, hence 2 d).
 """
-import math
+import threading
 
 import pytest
 import torch
@@ -127,6 +127,24 @@ def test_attention_waits_run_out(ops, L, H, d):
     assert int(flag) == 0
     for x, y in zip(first, again):
         assert torch.equal(x, y)
+
+
+def test_first_call_of_a_thread(ops):
+    """A thread whose first use of CUDA is one of the calls (its memory comes from the allocator's cache): the
+    results are the main thread's."""
+    q, k, v, ld, s0 = inputs(1, 200, 2, 64, 64, BF, s0=True)
+    x = torch.randn(2, 100, device="cuda")
+    calls = [lambda: ops.linear_attention_bwd(q, k, v, ld, v, initial_state=s0), lambda: ops.linear_attention(q, k, v, ld, return_final_state=True),
+             lambda: ops.qk_norm_rope(q, k), lambda: (ops.sample_tokens(x, x[:, 0].abs() % 1),),
+             lambda: ops.qk_norm_rope_bwd(q, k, ld.new_ones(64), ld.new_ones(64), v, v)]
+    for go in calls:
+        main = [t.clone() for t in go()]
+        got = []
+        thread = threading.Thread(target=lambda: got.extend(go()))
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert len(got) == len(main) and all(torch.equal(a, b) for a, b in zip(main, got))
 
 
 def test_attention_refusals(ops):
