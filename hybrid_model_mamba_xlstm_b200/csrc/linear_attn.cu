@@ -13,7 +13,7 @@
 namespace hxm {
 namespace lattn {
 
-constexpr int kTileV = 32;  // value columns per CTA
+constexpr int kSMs = 148;
 
 struct GenericParams {
   Common c;
@@ -24,26 +24,70 @@ struct GenericParams {
 // product n * log2(g) would lose the factor's low bits.
 HXM_DEV float decay_pow(double lg2, int n) { return n == 0 ? 1.f : (float)exp2(lg2 * n); }
 
-// One CTA: (batch, head), kTileV value columns, one time segment, in chunks of C steps held in shared
-// memory as fp32.  All sums are fp32 FMAs, so fp32 inputs keep their precision; per step and head
-// that is 2 C dk + 2 C dv + 4 dk dv operations on the FP32 pipe.
+// Rows 0 .. C - 1 of a chunk to shared memory as fp32: row r is time t0 + r * dt (r < nc), `cols` columns, zeros
+// elsewhere up to `pitch` (a multiple of 4).  Aligned fp32 rows by 16-byte copies that all are on their way at
+// once (the caller waits), others eight elements a thread at a time.
 template <typename T, int C>
+HXM_DEV void load_rows(float* dst, int ld, int pitch, const T* src, int64_t stride, int64_t t0, int dt, int nc, int cols) {
+  if (sizeof(T) == 4 && cols % 4 == 0 && stride % 4 == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+    const int pv = pitch / 4;
+    for (int i = threadIdx.x; i < C * pv; i += 256) {
+      const int r = i / pv, d = 4 * (i - r * pv);
+      const bool in = r < nc && d < cols;
+      const T* from = in ? src + (t0 + (int64_t)r * dt) * stride + d : src;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst + r * ld + d)),
+                   "l"(from), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+    return;
+  }
+  constexpr int B = 8;
+  for (int i0 = threadIdx.x; i0 < C * pitch; i0 += 256 * B) {
+    T x[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + 256 * k, r = i / pitch, d = i - r * pitch;
+      x[k] = __ldg(src + (r < nc && d < cols ? (t0 + (int64_t)r * dt) * stride + d : t0 * stride));
+    }
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int i = i0 + 256 * k, r = i / pitch, d = i - r * pitch;
+      if (r < C) dst[r * ld + d] = r < nc && d < cols ? to_f32<T>(x[k]) : 0.f;
+    }
+  }
+}
+template <int N> struct Pairs { float2 v[N / 2]; };
+template <int N> HXM_DEV Pairs<N> pairs(const float* at) { return *reinterpret_cast<const Pairs<N>*>(at); }
+template <int N>
+HXM_DEV void fma_row(Pairs<N>& acc, float a, const Pairs<N>& x) {
+#pragma unroll
+  for (int m = 0; m < N / 2; ++m) acc.v[m] = __ffma2_rn(make_float2(a, a), x.v[m], acc.v[m]);
+}
+
+// One CTA: (batch, head), TV value columns, one time segment, in chunks of C steps held in shared
+// memory as fp32.  All sums are fp32 FMAs, so fp32 inputs keep their precision; per step and head
+// that is 2 C dk (for each TV columns) + 2 C dv + 4 dk dv operations on the FP32 pipe, which bounds it: each of
+// the 256 threads holds a tile of C / 16 rows by TV / 16 columns of the product at hand, so that a float4 of
+// shared memory serves C / 16 or TV / 16 FMAs for each of its elements.  8 x 2048 x 16 heads of 128, fp32: 1.15 ms,
+// of which the products take four fifths, at half of the pipe's rate (two warps a scheduler); 2 x 513 x 4 heads
+// of 64: 34 us, half of it joining the segments.
+template <typename T, int C, int TV>
 __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ GenericParams gp, int dkp, int state_only) {
+  constexpr int M = C / 16, N = TV / 16;
   const Common& cm = gp.c;
   const int b = blockIdx.z % cm.batch;
   const Problem& p = gp.p[blockIdx.z / cm.batch];
-  const int h = blockIdx.y, seg = blockIdx.x % cm.nseg, e0 = (blockIdx.x / cm.nseg) * kTileV;
+  const int h = blockIdx.y, seg = blockIdx.x % cm.nseg, e0 = (blockIdx.x / cm.nseg) * TV;
   if (e0 >= p.dv) return;
   const int ld = dkp + 4;  // row pitch of Q, K
   extern __shared__ __align__(16) float sh[];
-  float* Q = sh;                 // [C][ld]
-  float* K = Q + C * ld;         // [C][ld]
-  float* V = K + C * ld;         // [C][32]
-  float* W = V + C * kTileV;     // [C][32]: V times its row's weight in the state
-  float* X = W + C * kTileV;     // [dkp][32]
-  float* P = X + dkp * kTileV;   // [C][C + 4]
-  float* pw = P + C * (C + 4);   // [C + 1]: g^0 .. g^C
-  const int tid = threadIdx.x;
+  float* Q = sh;             // [C][ld]
+  float* K = Q + C * ld;     // [C][ld]
+  float* V = K + C * ld;     // [C][TV]; times each row's weight in the state once the output has it
+  float* X = V + C * TV;     // [dkp][TV]
+  float* P = X + dkp * TV;   // [C][C]
+  float* pw = P + C * C;     // [C + 1]: g^0 .. g^C
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, c0 = tx * N;
   const double lg2 = (double)cm.log_decay[h] * 1.4426950408889634;
   const int n = cm.lengths ? min(max(cm.lengths[b], 0), cm.seqlen) : cm.seqlen;
   const int u_lo = seg * cm.seg_len, u_hi = min(n, u_lo + cm.seg_len);
@@ -52,54 +96,59 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
   // the state entering the segment
   const int nprev = state_only || n == 0 ? 0 : min(seg, (n + cm.seg_len - 1) / cm.seg_len);
   const float f0 = state_only || !p.s0 ? 0.f : decay_pow(lg2, n == 0 ? 0 : u_lo + is) * p.s0_scale;
-  for (int i = tid; i < dkp * kTileV; i += 256) {
-    const int d = i / kTileV, e = e0 + i % kTileV;
-    float x = 0.f;
-    if (d < p.dk && e < p.dv) {
-      if (!state_only && p.s0) x = f0 * p.s0[b * p.s0s[0] + h * p.s0s[1] + d * p.s0s[2] + e * p.s0s[3]];
-      for (int r = 0; r < nprev; ++r)
-        x = fmaf(decay_pow(lg2, u_lo - (r + 1) * cm.seg_len),
-                 p.ws[((((int64_t)b * cm.heads + h) * (cm.nseg - 1) + r) * p.dk + d) * p.dv + e], x);
+  __shared__ float join[kSMs];  // the earlier segments' factors; there are fewer segments than SMs
+  for (int r = tid; r < nprev; r += 256) join[r] = decay_pow(lg2, u_lo - (r + 1) * cm.seg_len);
+  __syncthreads();
+  constexpr int B = 8;  // elements a thread has on their way (dkp * TV is a multiple of 128)
+  for (int i0 = tid; i0 < dkp * TV; i0 += 256 * B) {
+    float x[B], y[B];
+    auto live = [&](int k) { return (i0 + 256 * k) / TV < p.dk && e0 + (i0 + 256 * k) % TV < p.dv; };
+    // (absent elements read the first one: loads without branches, all on their way at once)
+#pragma unroll
+    for (int k = 0; k < B; ++k) x[k] = 0.f;
+    if (f0 != 0.f) {
+      const float* s0 = p.s0 + b * p.s0s[0] + h * p.s0s[1] + e0 * p.s0s[3];
+#pragma unroll
+      for (int k = 0; k < B; ++k) y[k] = __ldg(s0 + (live(k) ? (i0 + 256 * k) / TV * p.s0s[2] + (i0 + 256 * k) % TV * p.s0s[3] : 0));
+#pragma unroll
+      for (int k = 0; k < B; ++k) x[k] = live(k) ? f0 * y[k] : 0.f;
     }
-    X[i] = x;
+    for (int r = 0; r < nprev; ++r) {
+      const float* ws = p.ws + (((int64_t)b * cm.heads + h) * (cm.nseg - 1) + r) * p.dk * p.dv + e0;
+#pragma unroll
+      for (int k = 0; k < B; ++k) y[k] = __ldg(ws + (live(k) ? (i0 + 256 * k) / TV * p.dv + (i0 + 256 * k) % TV : 0));
+#pragma unroll
+      for (int k = 0; k < B; ++k) x[k] = live(k) ? fmaf(join[r], y[k], x[k]) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < B; ++k)
+      if (i0 + 256 * k < dkp * TV) X[i0 + 256 * k] = x[k];
   }
-  T* o = static_cast<T*>(p.o) + b * p.so[0] + h * p.so[2];
+  T* o = static_cast<T*>(p.o) + b * p.so[0] + h * p.so[2] + e0;
   const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + h * p.sq[2];
   const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + h * p.sk[2];
-  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2] + e0;
   if (!state_only) {  // rows past the sequence
     const int lo = max(n, u_lo), hi = min(cm.seqlen, u_lo + cm.seg_len);
-    for (int i = tid; i < (hi - lo) * kTileV; i += 256) {
-      const int e = e0 + i % kTileV;
-      if (e < p.dv) o[(int64_t)(lo + i / kTileV) * p.so[1] + e] = from_f32<T>(0.f);
-    }
+    for (int i = tid; i < (hi - lo) * TV; i += 256)
+      if (e0 + i % TV < p.dv) o[(int64_t)(lo + i / TV) * p.so[1] + i % TV] = from_f32<T>(0.f);
   }
   const bool last_seg = n == 0 ? seg == 0 : (u_lo < n && u_hi == n);
   for (int u0 = u_lo; u0 < u_hi; u0 += C) {
     const int nc = min(C, u_hi - u0);
     const bool fin = !state_only && u0 + nc == n;  // exponents of the last state in the last chunk
     const int endexp = fin ? nc - 1 + fs : nc;
+    const int64_t t0 = p.reverse ? n - 1 - u0 : u0;
+    const int dt = p.reverse ? -1 : 1;
     __syncthreads();
-    for (int i = tid; i < C * dkp; i += 256) {
-      const int r = i / dkp, d = i % dkp;
-      const bool ok = r < nc && d < p.dk;
-      const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
-      K[r * ld + d] = ok ? to_f32<T>(k[t * p.sk[1] + d]) : 0.f;
-      if (!state_only) Q[r * ld + d] = ok ? to_f32<T>(q[t * p.sq[1] + d]) : 0.f;
-    }
-    for (int i = tid; i < C * kTileV; i += 256) {
-      const int r = i / kTileV, e = e0 + i % kTileV;
-      const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
-      const float x = r < nc && e < p.dv ? to_f32<T>(v[t * p.sv[1] + e]) : 0.f;
-      V[i] = x;
-      W[i] = r < nc ? x * pw[endexp - r] : 0.f;
-    }
+    load_rows<T, C>(K, ld, dkp, k, p.sk[1], t0, dt, nc, p.dk);
+    if (!state_only) load_rows<T, C>(Q, ld, dkp, q, p.sq[1], t0, dt, nc, p.dk);
+    load_rows<T, C>(V, TV, TV, v, p.sv[1], t0, dt, nc, min(TV, p.dv - e0));
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     if (!state_only) {
       {  // P = (q_i . k_j) g^(i-j), j <= i
-        constexpr int M = C / 16;
-        const int ty = tid / 16, tx = tid % 16;
-        float acc[M][M] = {};
+        float2 acc[M][M] = {};
         for (int d = 0; d < dkp; d += 4) {
           float4 a[M], c[M];
 #pragma unroll
@@ -110,66 +159,97 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
 #pragma unroll
           for (int i = 0; i < M; ++i)
 #pragma unroll
-            for (int j = 0; j < M; ++j)
-              acc[i][j] = fmaf(a[i].x, c[j].x, fmaf(a[i].y, c[j].y, fmaf(a[i].z, c[j].z, fmaf(a[i].w, c[j].w, acc[i][j]))));
+            for (int j = 0; j <= i; ++j) {  // columns of a later block of 16 lie behind all of the rows
+              acc[i][j] = __ffma2_rn(make_float2(a[i].x, a[i].y), make_float2(c[j].x, c[j].y), acc[i][j]);
+              acc[i][j] = __ffma2_rn(make_float2(a[i].z, a[i].w), make_float2(c[j].z, c[j].w), acc[i][j]);
+            }
         }
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
           for (int j = 0; j < M; ++j) {
             const int r = ty + 16 * i, s = tx + 16 * j;
-            P[r * (C + 4) + s] = s <= r ? acc[i][j] * pw[r - s] : 0.f;
+            P[r * C + s] = s <= r ? (acc[i][j].x + acc[i][j].y) * pw[r - s] : 0.f;
           }
       }
       __syncthreads();
-      {  // out = scale (P V + g^i Q X)
-        constexpr int N = C / 8, TPR = kTileV / N;  // columns per thread, threads per row
-        const int r = tid / TPR, c0 = (tid % TPR) * N;
-        float a[N] = {}, x[N] = {};
-        for (int j = 0; j < nc; ++j) {
-          const float w = P[r * (C + 4) + j];
+      {  // out = scale (g^i Q X + P V)
+        Pairs<N> acc[M] = {};
+        for (int d = 0; d < dkp; d += 4) {
+          float4 a[M];
 #pragma unroll
-          for (int m = 0; m < N; ++m) a[m] = fmaf(w, V[j * kTileV + c0 + m], a[m]);
+          for (int i = 0; i < M; ++i) a[i] = *reinterpret_cast<const float4*>(Q + (ty + 16 * i) * ld + d);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const Pairs<N> x = pairs<N>(X + (d + m) * TV + c0);
+#pragma unroll
+            for (int i = 0; i < M; ++i) fma_row(acc[i], m == 0 ? a[i].x : m == 1 ? a[i].y : m == 2 ? a[i].z : a[i].w, x);
+          }
         }
-        for (int d = 0; d < p.dk; ++d) {
-          const float w = Q[r * ld + d];
 #pragma unroll
-          for (int m = 0; m < N; ++m) x[m] = fmaf(w, X[d * kTileV + c0 + m], x[m]);
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+          for (int m = 0; m < N / 2; ++m) acc[i].v[m] = __fmul2_rn(make_float2(pw[ty + 16 * i], pw[ty + 16 * i]), acc[i].v[m]);
+        for (int j = 0; j < nc; j += 4) {  // rows behind the last are zeros
+          float4 a[M];
+#pragma unroll
+          for (int i = 0; i < M; ++i) a[i] = *reinterpret_cast<const float4*>(P + (ty + 16 * i) * C + j);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const Pairs<N> x = pairs<N>(V + (j + m) * TV + c0);
+#pragma unroll
+            for (int i = 0; i < M; ++i) fma_row(acc[i], m == 0 ? a[i].x : m == 1 ? a[i].y : m == 2 ? a[i].z : a[i].w, x);
+          }
         }
-        if (r < nc) {
-          const int64_t t = p.reverse ? n - 1 - (u0 + r) : u0 + r;
 #pragma unroll
-          for (int m = 0; m < N; ++m)
-            if (e0 + c0 + m < p.dv) o[t * p.so[1] + e0 + c0 + m] = from_f32<T>(p.scale * fmaf(pw[r], x[m], a[m]));
+        for (int i = 0; i < M; ++i) {
+          const int r = ty + 16 * i;
+          if (r >= nc) continue;
+          T* row = o + (t0 + (int64_t)r * dt) * p.so[1] + c0;
+#pragma unroll
+          for (int m = 0; m < N / 2; ++m) {
+            if (e0 + c0 + 2 * m < p.dv) row[2 * m] = from_f32<T>(p.scale * acc[i].v[m].x);
+            if (e0 + c0 + 2 * m + 1 < p.dv) row[2 * m + 1] = from_f32<T>(p.scale * acc[i].v[m].y);
+          }
         }
       }
       __syncthreads();
     }
-    {  // X = g^endexp X + K^T W
-      const int e = (tid % 8) * 4;
-      for (int d = tid / 8; d < dkp; d += 32) {
-        float4 x = *reinterpret_cast<float4*>(X + d * kTileV + e);
-        const float f = pw[endexp];
-        x.x *= f; x.y *= f; x.z *= f; x.w *= f;
-        for (int j = 0; j < nc; ++j) {
-          const float w = K[j * ld + d];
-          const float4 y = *reinterpret_cast<const float4*>(W + j * kTileV + e);
-          x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
-        }
-        *reinterpret_cast<float4*>(X + d * kTileV + e) = x;
+    for (int i = tid; i < nc * TV; i += 256) V[i] *= pw[endexp - i / TV];
+    __syncthreads();
+    // X = g^endexp X + K^T V
+    const float f = pw[endexp];
+    for (int d = 4 * ty; d < dkp; d += 64) {
+      Pairs<N> acc[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[i] = pairs<N>(X + (d + i) * TV + c0);
+#pragma unroll
+        for (int m = 0; m < N / 2; ++m) acc[i].v[m] = __fmul2_rn(make_float2(f, f), acc[i].v[m]);
       }
+#pragma unroll 4
+      for (int j = 0; j < nc; ++j) {
+        const float4 a = *reinterpret_cast<const float4*>(K + j * ld + d);
+        const Pairs<N> x = pairs<N>(V + j * TV + c0);
+        fma_row(acc[0], a.x, x);
+        fma_row(acc[1], a.y, x);
+        fma_row(acc[2], a.z, x);
+        fma_row(acc[3], a.w, x);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<Pairs<N>*>(X + (d + i) * TV + c0) = acc[i];
     }
   }
   __syncthreads();
   if (state_only) {
     if (seg < cm.nseg - 1 && u_lo < n)
-      for (int i = tid; i < dkp * kTileV; i += 256) {
-        const int d = i / kTileV, e = e0 + i % kTileV;
+      for (int i = tid; i < dkp * TV; i += 256) {
+        const int d = i / TV, e = e0 + i % TV;
         if (d < p.dk && e < p.dv) p.ws[((((int64_t)b * cm.heads + h) * (cm.nseg - 1) + seg) * p.dk + d) * p.dv + e] = X[i];
       }
   } else if (p.sT && last_seg) {
-    for (int i = tid; i < dkp * kTileV; i += 256) {
-      const int d = i / kTileV, e = e0 + i % kTileV;
+    for (int i = tid; i < dkp * TV; i += 256) {
+      const int d = i / TV, e = e0 + i % TV;
       if (d < p.dk && e < p.dv) p.sT[b * p.sTs[0] + h * p.sTs[1] + d * p.sTs[2] + e * p.sTs[3]] = p.sT_scale * X[i];
     }
   }
@@ -178,16 +258,19 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
 // Rounded up so that rows stay float4-aligned.
 static int padded_dk(int dk) { return (dk + 3) / 4 * 4; }
 
-static size_t generic_smem(int C, int dkp) {
-  return sizeof(float) * ((size_t)2 * C * (dkp + 4) + 2 * C * kTileV + (size_t)dkp * kTileV + C * (C + 4) + C + 4);
+static size_t generic_smem(int C, int tv, int dkp) {
+  return sizeof(float) * ((size_t)2 * C * (dkp + 4) + C * tv + (size_t)dkp * tv + C * C + C + 4);
 }
+// 64-step chunks and 64 columns while Q, K, X of the padded dk fit the shared memory of an SM (dk up to 256), else
+// 32 and 32.
+static int generic_tile(int dk) { return generic_smem(64, 64, padded_dk(dk)) <= 227 * 1024 ? 64 : 32; }
 
 template <typename T, int C>
-static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int tiles, bool state_only, cudaStream_t st) {
-  const size_t smem = generic_smem(C, dkp);
-  HXM_CUDA_TRY(cudaFuncSetAttribute(generic_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const dim3 grid((unsigned)(tiles * gp.c.nseg), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
-  generic_kernel<T, C><<<grid, 256, smem, st>>>(gp, dkp, state_only ? 1 : 0);
+static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int dv, bool state_only, cudaStream_t st) {
+  const size_t smem = generic_smem(C, C, dkp);
+  HXM_CUDA_TRY(cudaFuncSetAttribute(generic_kernel<T, C, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const dim3 grid((unsigned)((dv + C - 1) / C * gp.c.nseg), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
+  generic_kernel<T, C, C><<<grid, 256, smem, st>>>(gp, dkp, state_only ? 1 : 0);
   return check_launch("hxm_linear_attn");
 }
 
@@ -200,18 +283,15 @@ static hxm_status launch_generic(const Common& c, const Problem* p, int np, hxm_
     dk = p[i].dk > dk ? p[i].dk : dk;
     dv = p[i].dv > dv ? p[i].dv : dv;
   }
-  const int dkp = padded_dk(dk), tiles = (dv + kTileV - 1) / kTileV;
-  // 64-step chunks while Q, K, X of the padded dk fit the shared memory of an SM, else 32
-  if (generic_smem(64, dkp) <= 227 * 1024)
-    return io == HXM_F32 ? launch_generic_c<float, 64>(gp, np, dkp, tiles, state_only, st)
-                         : launch_generic_c<__nv_bfloat16, 64>(gp, np, dkp, tiles, state_only, st);
-  return io == HXM_F32 ? launch_generic_c<float, 32>(gp, np, dkp, tiles, state_only, st)
-                       : launch_generic_c<__nv_bfloat16, 32>(gp, np, dkp, tiles, state_only, st);
+  const int dkp = padded_dk(dk);
+  if (generic_tile(dk) == 64)
+    return io == HXM_F32 ? launch_generic_c<float, 64>(gp, np, dkp, dv, state_only, st)
+                         : launch_generic_c<__nv_bfloat16, 64>(gp, np, dkp, dv, state_only, st);
+  return io == HXM_F32 ? launch_generic_c<float, 32>(gp, np, dkp, dv, state_only, st)
+                       : launch_generic_c<__nv_bfloat16, 32>(gp, np, dkp, dv, state_only, st);
 }
 
 // ---- checks, time segments, dispatch -------------------------------------------------------------
-
-constexpr int kSMs = 148;
 
 static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -219,7 +299,7 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // time; every segment but the last first sums its own k v^T (pass one), the others' sums are joined
 // when a segment starts.  Pass one and the joining cost about half a chunk's and a few chunks' time on
 // the tensor cores, so a segment has `least` chunks there (4); on the FP32 pipe a chunk takes so much
-// longer that one will do (2 x 513 x 4 heads of 64, fp32: 170 us uncut).
+// longer that one will do (2 x 513 x 4 heads of 64, fp32: 34 us; two chunks 54, uncut 98).
 static void set_segments(Common& c, int64_t ctas, int chunk, int least) {
   const int chunks = ceil_div(c.seqlen, chunk);
   int64_t want = ctas > 0 ? kSMs / ctas : 1;
@@ -306,8 +386,12 @@ static void bwd_problems(const hxm_linear_attn_bwd_args* a, Problem out[3]) {
 static bool plan(Common& c, const Problem* p, int np, hxm_dtype io) {
   bool tc = true;
   int64_t ctas = 0;
-  for (int i = 0; i < np; ++i) tc = tc && tc_ok(p[i], c.seqlen, io);
-  for (int i = 0; i < np; ++i) ctas += (int64_t)c.batch * c.heads * ceil_div(p[i].dv, tc ? 64 : kTileV);
+  int dk = 0;
+  for (int i = 0; i < np; ++i) {
+    tc = tc && tc_ok(p[i], c.seqlen, io);
+    dk = p[i].dk > dk ? p[i].dk : dk;
+  }
+  for (int i = 0; i < np; ++i) ctas += (int64_t)c.batch * c.heads * ceil_div(p[i].dv, tc ? 64 : generic_tile(dk));
   if (tc) set_segments(c, ctas, 128, 4);
   else set_segments(c, ctas, 64, 1);
   return tc;
