@@ -35,6 +35,9 @@ def require_cuda(*tensors, who: str):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # of tensors, so CUDA is initialised
+
+
 def stream_of(device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
@@ -55,7 +58,7 @@ _HERE = _Here()
 def on_device(device):
     """A context in which ``device`` is the current CUDA device (launches go to the current device's
     context, whatever stream they name); free when it already is."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == _device() else torch.cuda.device(device)
 
 
 def once_only(who):

@@ -116,6 +116,29 @@ def test_sizes(sample, B, V):
     check(sample, logits, u, 0.8, 50, 1.0, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [50257, 9001])
+def test_top_k_of_every_size(sample, V, dtype):
+    """top_k on both sides of every limit between the ways to find it (rows of an odd length, so that each begins
+    elsewhere in its 16 bytes), alone and with top_p and min_p."""
+    logits, u = make(5, V, dtype, seed=11)
+    logits[1, ::2] = -float("inf")
+    logits[2, 40:] = -float("inf")  # fewer logits than most of the top_k
+    logits[3] = logits[3].round()   # many equal ones
+    for K in (2, 39, 40, 41, 127, 128, 129, 255, 256, 257, 399, 400, 401, 512, 513, 1024, 2000, V - 1):
+        check(sample, logits, u, 1.0, K)
+        check(sample, logits, u, 0.8, K, 0.9, 0.001)
+
+
+def test_extreme_settings(sample):
+    """Temperatures at which one token or all of them share the weight, top_p and min_p at their ends."""
+    logits, u = make(6, 5003, seed=13)
+    logits[5, 7] = float("inf")
+    for T in (1e-38, 1e-20, 1e-3, 1e4, 1e30, float("inf")):
+        for K, P, M in ((0, 1.0, 0.0), (0, 0.7, 0.0), (60, 1.0, 0.0), (3000, 0.9, 0.5), (0, 1e-7, 0.0), (0, 1.0, 1.0)):
+            check(sample, logits, u, T, K, P, M)
+
+
 def test_ties(sample):
     """Equal logits: the lowest tokens stay, whole rows of one value, few values, and greedy ties."""
     V = 5000
