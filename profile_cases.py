@@ -18,6 +18,10 @@ cases (default sizes):
   scan_bwd     B L D             (8 2048 2048)   selective-scan backward, bf16 inputs, fp32 gradients
   slstm        B L H HD          (8 256 4 256)    recurrent R
   conv         B D L             (8 4096 2048)    causal depthwise conv1d(4) + SiLU
+  linear_attn  B L H D           (8 2048 16 128)  linear attention with a decay per head, bf16, state in and out
+  linear_attn_step B H D         (128 16 128)     its single-token step
+  qk_norm_rope B L HQ HK D       (8 2048 16 4 128) norms of q's and k's heads with the rotation, bf16
+  sample       B V               (256 50304)      temperature 0.8, top_p 0.9, bf16 logits
   mamba_layer  B L               (8 2048)         one hybrid-350M Mamba block
   prefill      B L               (8 2048)         the hybrid-350M model forward
   prefill_graph B L PIECES       (8 2048 4)       the same prefill as a wavefront replayed from a CUDA graph
@@ -113,6 +117,34 @@ def main(argv=None):
         bias = torch.randn(D, generator=g, device=dev) * 0.1
         fn = lambda: causal_conv1d(x, w, bias, activation="silu")  # noqa: E731
         extra = {"bytes": 2 * x.numel() * 2}
+    elif a.case in ("linear_attn", "linear_attn_step", "qk_norm_rope", "sample"):
+        from hybrid_model_mamba_xlstm_b200 import kernels as K
+        g = torch.Generator(device=dev)
+        g.manual_seed(0)
+        rand = lambda *n: torch.randn(*n, generator=g, device=dev)  # noqa: E731
+        if a.case == "linear_attn":
+            B, L, H, D = (s + [8, 2048, 16, 128][len(s):])[:4]
+            q, k, v = (rand(B, L, H, D).to(torch.bfloat16) for _ in range(3))
+            s0, ld = rand(B, H, D, D), -torch.exp2(-3 - 7 * torch.arange(H, device=dev) / H)
+            fn = lambda: K.linear_attention(q, k, v, ld, initial_state=s0, return_final_state=True)  # noqa: E731
+            extra = {"bytes": 8 * q.numel() + 8 * s0.numel(), "flops": 4 * q.numel() * D}
+        elif a.case == "linear_attn_step":
+            B, H, D = (s + [128, 16, 128][len(s):])[:3]
+            q, k, v = (rand(B, H, D).to(torch.bfloat16) for _ in range(3))
+            s0, ld = rand(B, H, D, D), -torch.exp2(-3 - 7 * torch.arange(H, device=dev) / H)
+            fn = lambda: K.linear_attention_step(q, k, v, ld, s0)  # noqa: E731
+            extra = {"bytes": 8 * s0.numel()}
+        elif a.case == "qk_norm_rope":
+            B, L, HQ, HK, D = (s + [8, 2048, 16, 4, 128][len(s):])[:5]
+            q, k = rand(B, L, HQ, D).to(torch.bfloat16), rand(B, L, HK, D).to(torch.bfloat16)
+            w, pos = torch.ones(D, device=dev), torch.arange(L, device=dev)
+            fn = lambda: K.qk_norm_rope(q, k, w, w, pos)  # noqa: E731
+            extra = {"bytes": 4 * (q.numel() + k.numel())}
+        else:
+            B, V = (s + [256, 50304][len(s):])[:2]
+            logits, u = (2.5 * rand(B, V)).to(torch.bfloat16), torch.rand(B, generator=g, device=dev)
+            fn = lambda: K.sample_tokens(logits, u, temperature=0.8, top_p=0.9)  # noqa: E731
+            extra = {"bytes": 2 * logits.numel()}
     elif a.case in ("mamba_layer", "prefill"):
         from hybrid_model_mamba_xlstm_b200 import layers as Lyr
         B, L = (s + [8, 2048][len(s):])[:2]
