@@ -68,11 +68,12 @@ HXM_DEV void fma_row(Pairs<N>& acc, float a, const Pairs<N>& x) {
 // memory as fp32.  All sums are fp32 FMAs, so fp32 inputs keep their precision; per step and head
 // that is 2 C dk (for each TV columns) + 2 C dv + 4 dk dv operations on the FP32 pipe, which bounds it: each of
 // the 256 threads holds a tile of C / 16 rows by TV / 16 columns of the product at hand, so that a float4 of
-// shared memory serves C / 16 or TV / 16 FMAs for each of its elements.  8 x 2048 x 16 heads of 128, fp32: 1.15 ms,
-// of which the products take four fifths, at half of the pipe's rate (two warps a scheduler); 2 x 513 x 4 heads
-// of 64: 34 us, half of it joining the segments.
+// shared memory serves C / 16 or TV / 16 FMAs for each of its elements.  8 x 2048 x 16 heads of 128, fp32: 1.10 ms,
+// of which the products take four fifths, at half of the pipe's rate: a warp's 16-byte read takes four cycles of
+// shared memory, and eight of them serve 64 FMAs a thread.  2 x 513 x 4 heads of 64: 34 us, half of it joining the
+// segments.
 template <typename T, int C, int TV>
-__global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ GenericParams gp, int dkp, int state_only) {
+__global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__ GenericParams gp, int dkp, int state_only) {
   constexpr int M = C / 16, N = TV / 16;
   const Common& cm = gp.c;
   const int b = blockIdx.z % cm.batch;
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
     if (!state_only) {
       {  // P = (q_i . k_j) g^(i-j), j <= i
         float2 acc[M][M] = {};
+#pragma unroll 2
         for (int d = 0; d < dkp; d += 4) {
           float4 a[M], c[M];
 #pragma unroll
@@ -175,6 +177,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
       __syncthreads();
       {  // out = scale (g^i Q X + P V)
         Pairs<N> acc[M] = {};
+#pragma unroll 2
         for (int d = 0; d < dkp; d += 4) {
           float4 a[M];
 #pragma unroll
@@ -190,6 +193,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ Ge
         for (int i = 0; i < M; ++i)
 #pragma unroll
           for (int m = 0; m < N / 2; ++m) acc[i].v[m] = __fmul2_rn(make_float2(pw[ty + 16 * i], pw[ty + 16 * i]), acc[i].v[m]);
+#pragma unroll 2
         for (int j = 0; j < nc; j += 4) {  // rows behind the last are zeros
           float4 a[M];
 #pragma unroll
@@ -263,7 +267,7 @@ static size_t generic_smem(int C, int tv, int dkp) {
 }
 // 64-step chunks and 64 columns while Q, K, X of the padded dk fit the shared memory of an SM (dk up to 256), else
 // 32 and 32.
-static int generic_tile(int dk) { return generic_smem(64, 64, padded_dk(dk)) <= 227 * 1024 ? 64 : 32; }
+static int generic_tile(int dk) { return generic_smem(64, 64, padded_dk(dk)) + sizeof(float) * kSMs <= 227 * 1024 ? 64 : 32; }
 
 template <typename T, int C>
 static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int dv, bool state_only, cudaStream_t st) {

@@ -175,7 +175,7 @@ class LinearAttentionFunction(torch.autograd.Function):
 
 def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_state=None, return_final_state=False,
                      error_flag=None, wait_limit_cycles=0):
-    """Linear attention over whole sequences, from and to a carried state; differentiable.
+    """Linear attention over whole sequences, from and to a carried state; differentiable (once).
 
     q, k (B, L, H, dk), v (B, L, H, dv): bf16 or fp32, any strides (views with a unit last stride and
     16-byte aligned rows are read in place, zero strides too, others copied); log_decay (H,) fp32, at
@@ -208,7 +208,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
 def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
     """One step for every row: ``state`` (B, H, dk, dv; fp32, unit last stride) becomes
     exp(log_decay) state + k v^T in place, and o = scale * state^T q (B, H, dv) is returned (in ``out``
-    if given).  q, k (B, H, dk), v (B, H, dv): bf16 or fp32.  Without gradients."""
+    if given, which shares no memory with q, k or the state).  q, k (B, H, dk), v (B, H, dv): bf16 or fp32.
+    Without gradients."""
     who = "linear_attention_step"
     dev = require_cuda(q, k, v, log_decay, state, out, who=who)
     if q.dim() != 3:

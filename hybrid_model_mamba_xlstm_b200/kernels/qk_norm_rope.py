@@ -114,7 +114,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, *, rope_bas
     """RMS norm over the last dim of every head of q (B, L, Hq, d) and k (B, L, Hk, d), then the rotation of
     its first ``rotary_dim`` elements (default: all with positions, none without) by the position of the
     token: pair p turns by positions * rope_base**(-2p / rotary_dim), where a pair is elements p and
-    p + rotary_dim/2, or 2p and 2p + 1 with ``interleaved``.  Differentiable in q, k and the weights.
+    p + rotary_dim/2, or 2p and 2p + 1 with ``interleaved``.  Differentiable (once) in q, k and the weights.
 
     q, k: fp32, bf16 or fp16, read in place with any strides that have a unit last one (the column blocks of
     one projection's output); weights (d,) or None (ones); positions (B, L) or (L,) integers, the angles
