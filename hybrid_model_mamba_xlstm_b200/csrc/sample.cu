@@ -154,7 +154,7 @@ template <> struct Key<__nv_bfloat16> : Key16<__nv_bfloat16> {};
 template <> struct Key<__half> : Key16<__half> {};
 
 struct Shared {
-  double pow2[kTab];  // 2^(j / kTab)
+  double pow2[kTab];  // 2^44 2^(j / kTab)
   u64 scan[32];     // by warp; the rest stay 0
   u64 mine[2][2];   // this CTA's totals, double-buffered, for the cluster to read
   u64 sub[kMaxRuns];

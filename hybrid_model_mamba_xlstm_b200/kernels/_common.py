@@ -17,18 +17,18 @@ def dtype_code(t: torch.Tensor) -> int:
 
 def require_cuda(*tensors, who: str):
     """The kernels run only on a CUDA device; there is no CPU fallback."""
-    dev = None
+    first = index = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"{who}: tensors must be on a CUDA device (got {t.device}); "
                                "this package has no CPU path")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{who}: tensors on different devices ({dev} vs {t.device})")
-    return dev
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
+            raise RuntimeError(f"{who}: tensors on different devices ({first.device} vs {t.device})")
+    return None if first is None else first.device
 
 
 # The raw cudaStream_t of a device's current stream: the Stream object around it costs 2 us a call.

@@ -49,7 +49,7 @@ def _decay(who, log_decay, heads):
         raise ValueError(f"{who}: log_decay must be ({heads},), got {tuple(log_decay.shape)}")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{who}: log_decay is a constant; it must not require a gradient")
-    return log_decay.float().contiguous()
+    return log_decay if log_decay.dtype == torch.float32 and log_decay.is_contiguous() else log_decay.float().contiguous()
 
 
 def _rows(t):
@@ -221,14 +221,20 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
     _check_io(who, q, k, v)
     if state.shape != (bsz, nh, dk, dv) or state.dtype != torch.float32:
         raise ValueError(f"{who}: state must be fp32 {(bsz, nh, dk, dv)}, got {state.dtype} {tuple(state.shape)}")
-    if (dv > 1 and state.stride(-1) != 1) or any(s == 0 for s, n in zip(state.stride(), state.shape) if n > 1):
+    at = state.stride()
+    if (dv > 1 and at[3] != 1) or (bsz > 1 and at[0] == 0) or (nh > 1 and at[1] == 0) or (dk > 1 and at[2] == 0):
         raise ValueError(f"{who}: state is updated in place: it needs a unit last stride and no repeated rows")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or state.requires_grad):
         raise ValueError(f"{who}: has no gradient; use linear_attention, or torch.no_grad()")
     scale = _scale(who, scale, dk)
     with on_device(dev):
-        unit = lambda t: t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-        q, k, v = unit(q), unit(k), unit(v)
+        if dk > 1 and q.stride(2) != 1:
+            q = q.contiguous()
+        if dk > 1 and k.stride(2) != 1:
+            k = k.contiguous()
+        if dv > 1 and v.stride(2) != 1:
+            v = v.contiguous()
         ld = _decay(who, log_decay, nh)
         if out is None:
             out = torch.empty(bsz, nh, dv, device=dev, dtype=q.dtype)
@@ -237,6 +243,6 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
             raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride and no repeated rows")
         a = _step_args(_STEP, bsz, nh, dk, dv, dtype_code(q), q.data_ptr(), *q.stride()[:2], k.data_ptr(), *k.stride()[:2],
                        v.data_ptr(), *v.stride()[:2], out.data_ptr(), *out.stride()[:2], ld.data_ptr(), state.data_ptr(),
-                       *state.stride()[:3], scale)
+                       *at[:3], scale)
         _lib.call("hxm_linear_attn_step", a, stream_of(dev))
     return out

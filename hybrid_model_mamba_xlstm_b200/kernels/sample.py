@@ -2,12 +2,17 @@
 (hybrid_xmamba/models/hybrid_lm.py:238-262) in one launch, from given uniform numbers."""
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 
 from .. import _lib
-from ._common import dtype_code, on_device, ptr, require_cuda, stream_of
+from ._common import dtype_code, on_device, require_cuda, stream_of
 
 __all__ = ["sample_tokens"]
+
+_args, _SIZE = _lib.packer(_lib.SampleArgs), ctypes.sizeof(_lib.SampleArgs)
 
 
 def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, min_p=None, return_logprob=False):
@@ -25,44 +30,46 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, 
     logits: fp32, bf16 or fp16 with a unit last stride (others are copied), V <= 2^18.  Returns tokens (B,)
     [and the log-probability of each under the kept tokens, fp32: 0 when greedy, -inf for -1]."""
     who = "sample_tokens"
-    rows = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
-    tensors = {n: x for n, x in rows.items() if isinstance(x, torch.Tensor)}
-    dev = require_cuda(logits, uniforms, *tensors.values(), who=who)
+    rows = [x for x in (temperature, top_k, top_p, min_p) if isinstance(x, torch.Tensor)]
+    dev = require_cuda(logits, uniforms, *rows, who=who)
     if logits.dim() != 2 or uniforms.shape != logits.shape[:1]:
         raise ValueError(f"{who}: logits must be (B, V) and uniforms (B,), got {tuple(logits.shape)}, {tuple(uniforms.shape)}")
     bsz, vocab = logits.shape
     if vocab < 1:
         raise ValueError(f"{who}: empty vocabulary")
-    a = _lib.SampleArgs()
-    a.rows, a.vocab, a.io_dtype = bsz, vocab, dtype_code(logits)
-    off = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
     with on_device(dev):
-        keep = []
-        for n, x in rows.items():
-            if n in tensors:
+        keep = []  # the settings' tensors as the kernel reads them
+
+        def setting(name, x, off, most):
+            """(number, address of the numbers of the rows or 0)"""
+            if isinstance(x, torch.Tensor):
                 if x.shape != (bsz,):
-                    raise ValueError(f"{who}: {n} must be a number or ({bsz},), got {tuple(x.shape)}")
-                if n == "top_k" and (x.is_floating_point() or x.dtype == torch.bool):
-                    raise TypeError(f"{who}: top_k must be integers, got {x.dtype}")
-                x = (x if x.dtype == torch.int32 else x.clamp(0, vocab).int()) if n == "top_k" else x.float()
-                x = x.contiguous()
-                keep.append(x)
-                setattr(a, n + "_rows", x.data_ptr())
-                continue
-            x = off[n] if x is None else x
-            if n == "top_k":
+                    raise ValueError(f"{who}: {name} must be a number or ({bsz},), got {tuple(x.shape)}")
+                if name == "top_k":
+                    if x.is_floating_point() or x.dtype == torch.bool:
+                        raise TypeError(f"{who}: top_k must be integers, got {x.dtype}")
+                    x = x if x.dtype == torch.int32 else x.clamp(0, vocab).int()
+                keep.append((x if name == "top_k" else x.float()).contiguous())
+                return off, keep[-1].data_ptr()
+            if x is None:
+                return off, 0
+            if name == "top_k":
                 if x != int(x) or x < 0:
                     raise ValueError(f"{who}: top_k must be a whole number of at least 0, got {x}")
-                x = min(int(x), vocab)
-            elif not x >= 0 or (n != "temperature" and x > 1):
-                raise ValueError(f"{who}: {n} must be at least 0{'' if n == 'temperature' else ' and at most 1'}, got {x}")
-            setattr(a, n, x)
+                return min(int(x), vocab), 0
+            if not 0 <= x <= most:
+                raise ValueError(f"{who}: {name} must be at least 0{'' if name == 'temperature' else ' and at most 1'}, got {x}")
+            return ctypes.c_float(x).value, 0
+
+        settings = (*setting("temperature", temperature, 1.0, math.inf), *setting("top_k", top_k, 0, None),
+                    *setting("top_p", top_p, 1.0, 1), *setting("min_p", min_p, 0.0, 1))
         if vocab > 1 and logits.stride(1) != 1:
             logits = logits.contiguous()
-        uniforms = uniforms.float().contiguous()
+        if uniforms.dtype != torch.float32 or not uniforms.is_contiguous():
+            uniforms = uniforms.float().contiguous()
         tokens = torch.empty(bsz, device=dev, dtype=torch.int64)
         logprob = torch.empty(bsz, device=dev, dtype=torch.float32) if return_logprob else None
-        a.logits, a.logits_row_stride, a.uniforms = ptr(logits), logits.stride(0), ptr(uniforms)
-        a.tokens, a.logprob = ptr(tokens), ptr(logprob)
+        a = _args(_SIZE, bsz, vocab, dtype_code(logits), logits.data_ptr(), logits.stride(0), uniforms.data_ptr(), *settings,
+                  tokens.data_ptr(), logprob.data_ptr() if return_logprob else 0)
         _lib.call("hxm_sample_tokens", a, stream_of(dev))
     return (tokens, logprob) if return_logprob else tokens
