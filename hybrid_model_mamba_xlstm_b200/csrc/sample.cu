@@ -7,8 +7,8 @@
 // keys (16 bits for 16-bit logits).  What is left is a chain of passes over shared memory, bound by the
 // instructions issued (some 30 a token where a 64-bit weight is formed) and, for few rows, by the meetings
 // of the cluster between them:
-//   - small top_k: the k-th largest of the threads' own largest logits is a lower bound of the border, so one
-//     pass lists a few more than k tokens, which alone are ranked, cut and drawn from;
+//   - small top_k: the threads' own largest logits give a lower bound of the border, so one pass lists a few more
+//     than k tokens, which alone are ranked, cut and drawn from;
 //   - larger top_k: counts of the logits in 2048 bins, 1/64 of exp's unit wide, give the border's bin, and its
 //     keys are listed;
 //   - top_p: the weights' sums in the bins are right to 1 part in 10^4, so the border lies in a bin or a few; a
@@ -17,7 +17,7 @@
 //     pass; so are all keys where the list would not fit (logits of few values);
 //   - the draw: sums of runs of 128 tokens (of which the pass before has most already), the run that holds the
 //     target, the token in it.
-// 256 x 50304 bf16, GPU time: greedy 16 us, top_k 50 27, all tokens 40, top_p 0.9 82; 1 x 50304 fp32: 7, 13,
+// 256 x 50304 bf16, GPU time: greedy 16 us, top_k 50 25, all tokens 40, top_p 0.9 82; 1 x 50304 fp32: 7, 12,
 // 10 and 22; 32 x 131072 fp32, top_p 0.9: 41.
 //
 // Weights w = exp((logit - max) / temperature) are formed in 64 bits and held as integers of 2^-44:
@@ -760,14 +760,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     c.cl.sync();
   };
   if (k > 0 && k < p.vocab) {
-    // The k-th largest of the threads' own largest ones is no more than the k-th of all: with few enough
-    // keys above its bin, counts of those 512 a CTA do, and all tokens are looked at once.  Up to a quarter
-    // of them, some 10 % more than k pass; a longer list, or a larger k, takes counts of all tokens.
-    for (int pass = k <= kThreads / 4 * (int)c.cl.num_blocks() && k <= kTopKList ? 0 : 1; pass < 2; ++pass) {
+    // Where every CTA has k / CTAs threads whose own largest logit lies in its bin `last` or above, k tokens do: a lower
+    // bound of the border from 512 logits a CTA, for one look at all of them.  Up to a quarter of the threads, few more
+    // than k tokens pass; a longer list, or a larger k, takes counts of all tokens.
+    const int nb = (int)c.cl.num_blocks();
+    for (int pass = k <= kThreads / 4 * nb && k <= kTopKList ? 0 : 1; pass < 2; ++pass) {
       if (!clean) clear();
       clean = false;
+      int last, ahead = 0, listed = 0;
       if (pass == 0) {
         if (own) atomicAdd(&bins->n[place_of(c, own) >> 10], 1u);
+        if (tid == 0) sh.pick = kBins - 1;
+        __syncthreads();
+        const uint4 x = reinterpret_cast<const uint4*>(bins->n)[tid];
+        const uint32_t cnt[4] = {x.x, x.y, x.z, x.w}, share = (uint32_t)(k + nb - 1) / nb;
+        const uint32_t four = x.x + x.y + x.z + x.w;
+        uint32_t run = (uint32_t)block_prefix(&sh, four) - four;
+        for (int j = 0; j < 4; ++j) {
+          if (run < share && share <= run + cnt[j]) sh.pick = 4 * tid + j;
+          run += cnt[j];
+        }
+        c.cl.sync();
+        last = (int)__reduce_max_sync(0xffffffffu, lane < nb ? (uint32_t)*c.cl.map_shared_rank(&sh.pick, lane) : 0u);
+        if (last == kBins - 1) continue;  // a CTA with fewer logits, or too far below the largest
       } else {
         each_key(c, [&](const uint32_t (&key)[kBatch], int) {
           uint32_t at[kBatch];
@@ -777,32 +792,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
           for (int j = 0; j < kBatch; ++j)
             if (key[j]) atomicAdd(&bins->n[at[j]], 1u);
         });
-      }
-      uint32_t cnt[4];
-      read_bins(c, cnt);
-      const uint32_t four = cnt[0] + cnt[1] + cnt[2] + cnt[3];
-      const uint32_t upto = (uint32_t)block_prefix(&sh, four), from = upto - four;
-      __syncthreads();
-      if (tid == kThreads - 1) sh.pick = (int)upto;
-      __syncthreads();
-      const int valid = sh.pick;
-      if (k >= valid) {  // all of them stay; fewer largest ones than k say nothing
-        if (pass) k = 0;
-        continue;
-      }
-      __syncthreads();
-      uint32_t run = from;
-      for (int j = 0; j < 4; ++j) {
-        if (run < (uint32_t)k && (uint32_t)k <= run + cnt[j]) {
-          sh.pick = 4 * tid + j;
-          sh.pick2 = (int)(run + cnt[j]);
-          sh.run_at = (int)run;  // tokens before the bin
+        uint32_t cnt[4];
+        read_bins(c, cnt);
+        const uint32_t four = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+        const uint32_t upto = (uint32_t)block_prefix(&sh, four), from = upto - four;
+        __syncthreads();
+        if (tid == kThreads - 1) sh.pick = (int)upto;
+        __syncthreads();
+        if (k >= sh.pick) {  // all of them stay
+          k = 0;
+          continue;
         }
-        run += cnt[j];
+        __syncthreads();
+        uint32_t run = from;
+        for (int j = 0; j < 4; ++j) {
+          if (run < (uint32_t)k && (uint32_t)k <= run + cnt[j]) {
+            sh.pick = 4 * tid + j;
+            sh.pick2 = (int)(run + cnt[j]);
+            sh.run_at = (int)run;  // tokens before the bin
+          }
+          run += cnt[j];
+        }
+        __syncthreads();
+        last = sh.pick;
+        listed = sh.pick2;
+        ahead = sh.run_at;
       }
-      __syncthreads();
-      const int last = sh.pick, ahead = sh.run_at;
-      int listed = sh.pick2;
       if (pass == 0 || (k <= kTopKList && listed <= kList)) {
         gather(c, i0, bin_floor(c, last));
         c.cl.sync();
