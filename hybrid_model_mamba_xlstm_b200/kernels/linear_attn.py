@@ -99,7 +99,7 @@ def _forward(q, k, v, log_decay, scale, lengths, s0, want_state, error_flag=None
     dev = require_cuda(q, k, v, log_decay, lengths, s0, error_flag, who=who)
     with on_device(dev):
         _check(who, q, k, v)
-        out = torch.empty(v.shape, device=dev, dtype=q.dtype)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
         sT = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], device=dev, dtype=torch.float32) if want_state else None
         a, keep = _fill(who, q, k, v, log_decay, scale, lengths, s0, out, sT, error_flag, wait_limit_cycles)
         n = _lib.lib().hxm_linear_attn_workspace_size(a)
@@ -133,9 +133,9 @@ def linear_attention_bwd(q, k, v, log_decay, dout, *, scale=None, lengths=None, 
             if d_final_state.shape != sshape:
                 raise ValueError(f"{who}: d_final_state must be {sshape}, got {tuple(d_final_state.shape)}")
             d_final_state = d_final_state.float()
-        dq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dk = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        dv = torch.empty(v.shape, device=dev, dtype=q.dtype)
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         ds0 = torch.empty(sshape, device=dev, dtype=torch.float32) if need_d_initial_state else None
         a = _bwd_args(bytes(f), _BWD, *_at(dout),
                       *(_NONE if d_final_state is None else (d_final_state.data_ptr(), *d_final_state.stride())),
@@ -237,7 +237,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
             v = v.contiguous()
         ld = _decay(who, log_decay, nh)
         if out is None:
-            out = torch.empty(bsz, nh, dv, device=dev, dtype=q.dtype)
+            out = torch.empty_like(v, memory_format=torch.contiguous_format)
         elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1) or any(
                 s == 0 for s, n in zip(out.stride(), out.shape) if n > 1):
             raise ValueError(f"{who}: out must be {q.dtype} {(bsz, nh, dv)} with a unit last stride and no repeated rows")

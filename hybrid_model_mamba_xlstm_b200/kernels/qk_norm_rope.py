@@ -7,16 +7,20 @@ position-dependent angles in the same HBM pass.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
 from .. import _lib
-from ._common import dtype_code, f32_param, on_device, once_only, ptr, require_cuda, stream_of
+from ._common import dtype_code, f32_param, on_device, once_only, require_cuda, stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_bwd"]
 
 _fwd_args, _bwd_args = _lib.packer(_lib.QkNormRopeArgs), _lib.packer(_lib.QkNormRopeBwdArgs)
 _FWD, _BWD = ctypes.sizeof(_lib.QkNormRopeArgs), ctypes.sizeof(_lib.QkNormRopeBwdArgs)
+
+
+_IO = (torch.bfloat16, torch.float32, torch.float16)
 
 
 def _unit(t):
@@ -25,35 +29,43 @@ def _unit(t):
 
 def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
     """(args of the forward with new dense outputs, these, tensors to keep alive)."""
-    if q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[-1] != q.shape[-1]:
+    if q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
         raise ValueError(f"{who}: q must be (B, L, Hq, d) and k (B, L, Hk, d), got {tuple(q.shape)}, {tuple(k.shape)}")
-    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or k.dtype != q.dtype:
+    if q.dtype not in _IO or k.dtype != q.dtype:
         raise TypeError(f"{who}: q and k must both be fp32, bf16 or fp16, got {q.dtype}, {k.dtype}")
     bsz, L, hq, d = q.shape
-    for name, w in (("q_weight", qw), ("k_weight", kw)):
-        if w is not None and w.shape != (d,):
-            raise ValueError(f"{who}: {name} must be ({d},), got {tuple(w.shape)}")
+    hk = k.shape[2]
+    if qw is not None and qw.shape != (d,):
+        raise ValueError(f"{who}: q_weight must be ({d},), got {tuple(qw.shape)}")
+    if kw is not None and kw.shape != (d,):
+        raise ValueError(f"{who}: k_weight must be ({d},), got {tuple(kw.shape)}")
     rotary = (d - d % 2 if positions is not None else 0) if rotary is None else int(rotary)
     if rotary < 0 or rotary > d or rotary % 2:
         raise ValueError(f"{who}: rotary_dim must be even and at most {d}, got {rotary}")
-    if rotary and positions is None:
-        raise ValueError(f"{who}: a rotation needs positions")
-    if rotary and not (base > 0 and base < float("inf")):
-        raise ValueError(f"{who}: rope_base must be positive and finite, got {base}")
-    q, k = _unit(q), _unit(k)
     qw, kw = f32_param(qw), f32_param(kw)
     at = (0, 0, 0)
     if rotary:
-        if positions.is_floating_point() or positions.dtype == torch.bool or positions.shape not in ((bsz, L), (L,)):
-            raise ValueError(f"{who}: positions must be integers ({bsz}, {L}) or ({L},), got {positions.dtype} "
-                             f"{tuple(positions.shape)}")
-        positions = positions.long()
-        at = (positions.data_ptr(), *(positions.stride() if positions.dim() == 2 else (0, positions.stride(0))))
-    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    yk = torch.empty(k.shape, device=q.device, dtype=q.dtype)
-    a = _fwd_args(_FWD, bsz, L, hq, k.shape[2], d, rotary, dtype_code(q), bool(interleaved),
-                  q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], ptr(qw) or 0, ptr(kw) or 0, *at,
-                  float(base), float(eps), yq.data_ptr(), *yq.stride()[:3], yk.data_ptr(), *yk.stride()[:3])
+        if positions is None:
+            raise ValueError(f"{who}: a rotation needs positions")
+        if not 0 < base < math.inf:
+            raise ValueError(f"{who}: rope_base must be positive and finite, got {base}")
+        if positions.dtype != torch.int64:
+            if positions.is_floating_point() or positions.dtype == torch.bool:
+                raise ValueError(f"{who}: positions must be integers, got {positions.dtype}")
+            positions = positions.long()
+        if positions.shape == (bsz, L):
+            at = (positions.data_ptr(), *positions.stride())
+        elif positions.shape == (L,):
+            at = (positions.data_ptr(), 0, positions.stride(0))
+        else:
+            raise ValueError(f"{who}: positions must be ({bsz}, {L}) or ({L},), got {tuple(positions.shape)}")
+    q, k = _unit(q), _unit(k)
+    yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    yk = torch.empty_like(k, memory_format=torch.contiguous_format)
+    a = _fwd_args(_FWD, bsz, L, hq, hk, d, rotary, dtype_code(q), bool(interleaved),
+                  q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3],
+                  0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(), *at, base, eps,
+                  yq.data_ptr(), L * hq * d, hq * d, d, yk.data_ptr(), L * hk * d, hk * d, d)
     return a, yq, yk, (q, k, qw, kw, positions)
 
 
@@ -78,14 +90,12 @@ def qk_norm_rope_bwd(q, k, q_weight, k_weight, dq_out, dk_out, positions=None, *
     with on_device(dev):
         f, dq, dk, keep = _fill(who, q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)
         dq_out, dk_out = _unit(dq_out), _unit(dk_out)
-        d = q.shape[-1]
-        dw = [torch.empty(d, device=dev, dtype=torch.float32) if weight_grads and w is not None else None
-              for w in (q_weight, k_weight)]
+        dw = [torch.empty_like(w) if weight_grads and w is not None else None for w in keep[2:4]]
         a = _bwd_args(bytes(f), _BWD, dq_out.data_ptr(), *dq_out.stride()[:3], dk_out.data_ptr(), *dk_out.stride()[:3],
-                      ptr(dw[0]) or 0, ptr(dw[1]) or 0, 0, 0)
+                      0 if dw[0] is None else dw[0].data_ptr(), 0 if dw[1] is None else dw[1].data_ptr(), 0, 0)
         n = _lib.lib().hxm_qk_norm_rope_bwd_workspace_size(a)
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        a.workspace, a.workspace_bytes = ptr(ws), n
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
         _lib.call("hxm_qk_norm_rope_bwd", a, stream_of(dev))
     return dq, dk, dw[0], dw[1]
 
@@ -119,6 +129,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, *, rope_bas
     q, k: fp32, bf16 or fp16, read in place with any strides that have a unit last one (the column blocks of
     one projection's output); weights (d,) or None (ones); positions (B, L) or (L,) integers, the angles
     formed in 64 bits.  d <= 1024.  Returns the two results, dense, in q's dtype."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         return QkNormRopeFunction.apply(q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)
     return _forward(q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)

@@ -67,8 +67,8 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, 
             logits = logits.contiguous()
         if uniforms.dtype != torch.float32 or not uniforms.is_contiguous():
             uniforms = uniforms.float().contiguous()
-        tokens = torch.empty(bsz, device=dev, dtype=torch.int64)
-        logprob = torch.empty(bsz, device=dev, dtype=torch.float32) if return_logprob else None
+        tokens = torch.empty_like(uniforms, dtype=torch.int64)
+        logprob = torch.empty_like(uniforms) if return_logprob else None
         a = _args(_SIZE, bsz, vocab, dtype_code(logits), logits.data_ptr(), logits.stride(0), uniforms.data_ptr(), *settings,
                   tokens.data_ptr(), logprob.data_ptr() if return_logprob else 0)
         _lib.call("hxm_sample_tokens", a, stream_of(dev))
