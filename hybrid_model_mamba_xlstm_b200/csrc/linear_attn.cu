@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
     for (int r = 0; r < nprev; ++r) {
       const float* ws = p.ws + (((int64_t)b * cm.heads + h) * (cm.nseg - 1) + r) * p.dk * p.dv + e0;
 #pragma unroll
-      for (int k = 0; k < B; ++k) y[k] = __ldg(ws + (live(k) ? (i0 + 256 * k) / TV * p.dv + (i0 + 256 * k) % TV : 0));
+      for (int k = 0; k < B; ++k) y[k] = __ldg(ws + (live(k) ? (int64_t)((i0 + 256 * k) / TV) * p.dv + (i0 + 256 * k) % TV : 0));
 #pragma unroll
       for (int k = 0; k < B; ++k) x[k] = live(k) ? fmaf(join[r], y[k], x[k]) : 0.f;
     }

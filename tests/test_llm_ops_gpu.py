@@ -147,6 +147,61 @@ def test_first_call_of_a_thread(ops):
         assert len(got) == len(main) and all(torch.equal(a, b) for a, b in zip(main, got))
 
 
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F32, 128)])
+def test_attention_offsets_beyond_32_bits(ops, dtype, d):
+    """Over 2^31 elements: with no memory between steps (log_decay -inf) o = scale (q k) v for every step, which the last
+    rows show; the gradients there are those of the same rows alone."""
+    L, H, tail = 2 ** 31 // (16 * d) + 200, 16, 300
+    ld = torch.full((H,), -float("inf"), device="cuda")
+    big = [torch.zeros(1, L, H, d, device="cuda", dtype=dtype) for _ in range(3)]
+    small = inputs(1, tail, H, d, d, dtype, seed=1)[:3]
+    for x, y in zip(big, small):
+        x[:, -tail:] = y
+    q, k, v = (x.double() for x in small)
+    ref, size = 0.1 * (q * k).sum(-1, keepdim=True) * v, 0.1 * (q * k).abs().sum(-1, keepdim=True) * v.abs()
+    o = ops.linear_attention(*big, ld, scale=0.1)
+    unit = (d + 64) * 2.0 ** -24 * size + (2.0 ** -8 * (ref.abs() + size) if dtype == BF else 0)
+    assert bool(((o[:, -tail:].double() - ref).abs() <= unit).all()) and float(o[:, :-tail].abs().max()) == 0
+    del o
+    # chunks begin elsewhere in the long call: the same sums in another order, each product rounded apart
+    got = ops.linear_attention_bwd(*big, ld, big[2], scale=0.1)
+    want = ops.linear_attention_bwd(*small, ld, small[2], scale=0.1)
+    for x, y in zip(got[:3], want[:3]):
+        assert float((x[:, -tail:].double() - y.double()).norm() / y.double().norm()) <= (2.0 ** -7 if dtype == BF else (d + 64) * 2.0 ** -24)
+        assert float(x[:, :-tail].abs().max()) == 0
+
+
+def test_other_offsets_beyond_32_bits(ops):
+    """The last rows of over 2^31 elements of state, of heads and of logits are those of the same rows alone."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    B, H, d = 2 ** 31 // (16 * 128 * 128) + 3, 16, 128
+    state, ld = torch.zeros(B, H, d, d, device="cuda"), torch.full((H,), -0.1, device="cuda")
+    state[-2:] = r(2, H, d, d)
+    q, k, v, last = r(B, H, d), r(B, H, d), r(B, H, d), state[-2:].clone()
+    o, o2 = ops.linear_attention_step(q, k, v, ld, state), ops.linear_attention_step(q[-2:], k[-2:], v[-2:], ld, last)
+    assert torch.equal(o[-2:], o2) and torch.equal(state[-2:], last)
+    del state, o
+    L = 2 ** 31 // (16 * 128) + 5
+    x, w = torch.zeros(1, L, 16, 128, device="cuda", dtype=BF), 1 + 0.1 * r(128)
+    x[:, -9:] = r(1, 9, 16, 128).to(BF)
+    pos = torch.arange(L, device="cuda")
+    y, z = ops.qk_norm_rope(x, x[:, :, :1], w, w, pos)
+    y2, z2 = ops.qk_norm_rope(x[:, -9:], x[:, -9:, :1], w, w, pos[-9:])
+    assert torch.equal(y[:, -9:], y2) and torch.equal(z[:, -9:], z2)
+    dx, _, _, _ = ops.qk_norm_rope_bwd(x, x[:, :, :1], w, w, y, z, pos)
+    dx2, _, _, _ = ops.qk_norm_rope_bwd(x[:, -9:], x[:, -9:, :1], w, w, y2, z2, pos[-9:])
+    assert torch.equal(dx[:, -9:], dx2)
+    del x, y, z, dx
+    V = 50304
+    B = 2 ** 31 // V + 5
+    logits = torch.zeros(B, V, device="cuda", dtype=BF)
+    logits[-4:] = r(4, V).to(BF)
+    u = torch.rand(B, generator=g, device="cuda")
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9)):
+        assert torch.equal(ops.sample_tokens(logits, u, **kw)[-4:], ops.sample_tokens(logits[-4:], u[-4:], **kw))
+
+
 def test_attention_refusals(ops):
     q, k, v, ld, s0 = inputs(2, 9, 2, 16, 24, F32, s0=True)
     f, step = ops.linear_attention, ops.linear_attention_step
