@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kThreads) vec_kernel(const Params p) {
           float ssq = sq.x + sq.y;
 #pragma unroll
           for (int o = G / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-          const float2 inv = both(rsqrtf(fmaf(ssq, per_dim, p.eps)));
+          // a lane without a row adds nothing to the weight sums: there rsqrt would be infinite for eps = 0
+          const float2 inv = both(!BWD || hb + r * hs < rows ? rsqrtf(fmaf(ssq, per_dim, p.eps)) : 0.f);
           if (!BWD) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {

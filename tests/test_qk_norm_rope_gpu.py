@@ -217,3 +217,29 @@ def test_repeats_streams_graph(ops):
     torch.cuda.synchronize()
     late = torch.autograd.grad(alive, leaves, [torch.ones_like(t) for t in alive])
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, got, late))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("case", [(1, 5, 4, 3, 128, 128, False), (2, 37, 3, 1, 64, 32, True), (1, 1191, 3, 1, 64, 64, False),
+                                  (1, 3, 1, 2, 1024, 0, False), (1, 6, 2, 1, 37, 36, False)])
+def test_gradients_without_eps(ops, case, dtype):
+    """eps = 0: the formula is finite for rows that are not zero, and so are its gradients, with fewer heads than groups
+    of lanes and a last block that its tokens do not fill.  Tolerances as in test_gradients."""
+    B, L, hq, hk, d, rot, inter = case
+    q, k, wq, wk = make(B, L, hq, hk, d, dtype, seed=d + 2)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    gq = torch.randn(q.shape, generator=g, device="cuda").to(dtype)
+    gk = torch.randn(k.shape, generator=g, device="cuda").to(dtype)
+    pos = torch.randint(0, 4000, (B, L), device="cuda")
+    got = ops.qk_norm_rope_bwd(q, k, wq, wk, gq, gk, pos, rotary_dim=rot, interleaved=inter, eps=0.0)
+    rows = B * L * max(hq, hk)
+    for x, w, gy, gx, gw in ((q, wq, gq, got[0], got[2]), (k, wk, gk, got[1], got[3])):
+        lx, lw = x.double().requires_grad_(), w.double().requires_grad_()
+        rx, rw = torch.autograd.grad(ref_one(lx, lw, pos, 10000.0, rot, inter, 0.0), (lx, lw), gy.double())
+        inv = 1 / torch.sqrt((x.double() ** 2).mean(-1, keepdim=True))
+        n = x.double() * inv
+        size = 2 * inv * (gy.double().abs().amax(-1, keepdim=True) * 1.5 * w.abs().max() * (2 + n.abs() * n.abs().mean(-1, keepdim=True)))
+        tol = half_step(dtype) * rx.abs() + (d + 80) * 2.0 ** -24 * size + (2.0 ** -25 if dtype == F16 else 0)
+        assert bool(((gx.double() - rx).abs() <= tol).all())
+        sizes = (gy.double().abs().amax(-1, keepdim=True) * 1.5 * n.abs()).flatten(0, 2).sum(0)
+        assert bool(((gw.double() - rw).abs() <= (d / 2 + 40 + rows) * 2.0 ** -24 * sizes + 1e-30).all())
