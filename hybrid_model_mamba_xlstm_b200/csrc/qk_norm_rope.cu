@@ -439,6 +439,7 @@ static hxm_status check_args(const hxm_qk_norm_rope_args* a, const char* who) {
   HXM_REQUIRE(a->rotary >= 0 && a->rotary <= a->dim && a->rotary % 2 == 0, "%s: rotary %d must be even and at most dim %d", who,
               a->rotary, a->dim);
   HXM_REQUIRE(a->rotary == 0 || (a->rope_base > 0 && a->rope_base - a->rope_base == 0), "%s: rope_base must be positive and finite", who);
+  HXM_REQUIRE(a->eps >= 0 && a->eps - a->eps == 0, "%s: eps must be finite and at least 0", who);
   HXM_REQUIRE_SUPPORTED((int64_t)a->heads_q + a->heads_k <= (1 << 20), "%s: %lld heads", who, (long long)a->heads_q + a->heads_k);
   return HXM_OK;
 }

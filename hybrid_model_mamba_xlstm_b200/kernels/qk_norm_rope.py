@@ -42,6 +42,8 @@ def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
     rotary = (d - d % 2 if positions is not None else 0) if rotary is None else int(rotary)
     if rotary < 0 or rotary > d or rotary % 2:
         raise ValueError(f"{who}: rotary_dim must be even and at most {d}, got {rotary}")
+    if not 0 <= eps < math.inf:
+        raise ValueError(f"{who}: eps must be finite and at least 0, got {eps}")
     qw, kw = f32_param(qw), f32_param(kw)
     at = (0, 0, 0)
     if rotary:
@@ -128,7 +130,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, *, rope_bas
 
     q, k: fp32, bf16 or fp16, read in place with any strides that have a unit last one (the column blocks of
     one projection's output); weights (d,) or None (ones); positions (B, L) or (L,) integers, the angles
-    formed in 64 bits.  d <= 1024.  Returns the two results, dense, in q's dtype."""
+    formed in 64 bits.  d <= 1024; eps at least 0 (0: a row of zeros gives NaN, as the formula does).  Returns
+    the two results, dense, in q's dtype."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         return QkNormRopeFunction.apply(q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)

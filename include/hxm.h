@@ -663,7 +663,7 @@ hxm_status hxm_linear_attn_step(const hxm_linear_attn_step_args* args, void* str
 /* rotary), the angle formed in 64 bits.  x, out: element strides (b, t, h),   */
 /* unit stride in the last dim, fp32 / bf16 / fp16; weights fp32 (dim) or NULL */
 /* (ones); positions int64 with element strides (b, t), or NULL with rotary 0. */
-/* dim <= 1024.                                                                */
+/* dim <= 1024; eps finite, 0 or more (0: a row of zeros gives NaN).           */
 typedef struct hxm_qk_norm_rope_args {
   size_t struct_size;
   int32_t batch, seqlen, heads_q, heads_k, dim, rotary;

@@ -304,3 +304,12 @@ def test_generate_from_uniforms(ops, graph):
     assert drawn.shape == (2, 15) and 0 <= int(drawn.min()) and int(drawn.max()) < 97
     with pytest.raises(ValueError, match="uniforms"):
         model.generate(prompt, max_new_tokens=6, uniforms=u[:, :5])
+
+
+def test_norms_refuse_an_eps_that_is_none(ops):
+    q, w = torch.randn(2, 5, 4, 32, device="cuda"), torch.ones(32, device="cuda")
+    for eps in (-1e-6, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            ops.qk_norm_rope(q, q, w, w, eps=eps)
+        with pytest.raises(ValueError, match="eps"):
+            ops.qk_norm_rope_bwd(q, q, w, w, q, q, eps=eps)

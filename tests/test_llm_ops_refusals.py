@@ -135,3 +135,15 @@ def test_wrappers_on_cpu_tensors():
                lambda: kernels.sample_tokens(torch.zeros(2, 5), torch.zeros(2))):
         with pytest.raises(RuntimeError, match="CUDA device"):
             go()
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_norms_eps(eps):
+    a = _lib.QkNormRopeArgs()
+    a.batch, a.seqlen, a.heads_q, a.heads_k, a.dim, a.io_dtype, a.rope_base, a.eps = 1, 2, 2, 1, 64, _lib.HXM_F32, 1e4, eps
+    got, said = call("hxm_qk_norm_rope_fwd", a)
+    assert got == _lib.HXM_EBADARG and "eps" in said
+    b = _lib.QkNormRopeBwdArgs()
+    b.fwd = a
+    got, said = call("hxm_qk_norm_rope_bwd", b)
+    assert got == _lib.HXM_EBADARG and "eps" in said
