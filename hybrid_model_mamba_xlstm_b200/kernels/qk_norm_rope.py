@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from ._common import dtype_code, f32_param, on_device, once_only, require_cuda, stream_of
+from ._common import dtype_code, on_device, once_only, require_cuda, stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_bwd"]
 
@@ -25,6 +25,12 @@ _IO = (torch.bfloat16, torch.float32, torch.float16)
 
 def _unit(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _f32(w):
+    """A weight as the kernels read it.  A 16-bit one is widened at every call, on the call's stream: a copy kept
+    between calls would be blind to writes through .data and to those of other streams and replayed graphs."""
+    return w if w is None or (w.dtype == torch.float32 and w.is_contiguous()) else w.detach().float().contiguous()
 
 
 def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
@@ -44,7 +50,7 @@ def _fill(who, q, k, qw, kw, positions, base, rotary, interleaved, eps):
         raise ValueError(f"{who}: rotary_dim must be even and at most {d}, got {rotary}")
     if not 0 <= eps < math.inf:
         raise ValueError(f"{who}: eps must be finite and at least 0, got {eps}")
-    qw, kw = f32_param(qw), f32_param(kw)
+    qw, kw = _f32(qw), _f32(kw)
     at = (0, 0, 0)
     if rotary:
         if positions is None:

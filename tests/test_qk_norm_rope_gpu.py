@@ -243,3 +243,38 @@ def test_gradients_without_eps(ops, case, dtype):
         assert bool(((gx.double() - rx).abs() <= tol).all())
         sizes = (gy.double().abs().amax(-1, keepdim=True) * 1.5 * n.abs()).flatten(0, 2).sum(0)
         assert bool(((gw.double() - rw).abs() <= (d / 2 + 40 + rows) * 2.0 ** -24 * sizes + 1e-30).all())
+
+
+@pytest.mark.parametrize("wdtype", [BF, F16])
+def test_weights_of_16_bits_are_read_at_each_call(ops, wdtype):
+    """The result is that of the weights' values at the call (widened exactly): after a write that autograd's version
+    count does not see, for tensors without such a count, from another stream, and at each replay of a graph that was
+    captured after a first call."""
+    q, k, wq, wk = make(2, 9, 2, 1, 64, BF, seed=3)
+    pos = torch.arange(9, device="cuda")
+    wq, wk = wq.to(wdtype), wk.to(wdtype)
+    f = lambda: torch.cat([t.flatten() for t in ops.qk_norm_rope(q, k, wq, wk, pos)])
+    want = lambda: torch.cat([t.flatten() for t in ops.qk_norm_rope(q, k, wq.float(), wk.float(), pos)])
+    assert torch.equal(f(), want())
+    wq.data.mul_(2)
+    wk.data.add_(1)
+    assert torch.equal(f(), want())
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        wq.data.mul_(0.5)
+        got = f()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = f()
+    for _ in range(2):
+        wq.mul_(-2)
+        wk.data.mul_(0.5)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want())
+    with torch.inference_mode():
+        wq, wk = wq.clone(), wk.clone()
+        assert torch.equal(f(), want())
