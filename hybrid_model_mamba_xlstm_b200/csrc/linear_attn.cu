@@ -205,6 +205,20 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
             for (int i = 0; i < M; ++i) fma_row(acc[i], m == 0 ? a[i].x : m == 1 ? a[i].y : m == 2 ? a[i].z : a[i].w, x);
           }
         }
+        // An infinity or NaN in V reached the rows before it too (their weights are 0, and 0 * inf is NaN): sums that are
+        // not finite are formed again, from the steps up to their row alone.
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+          for (int m = 0; m < N; ++m) {
+            float& sum = m & 1 ? acc[i].v[m / 2].y : acc[i].v[m / 2].x;
+            if (sum - sum == 0.f) continue;
+            const int r = ty + 16 * i;
+            sum = 0.f;
+            for (int d = 0; d < dkp; ++d) sum = fmaf(Q[r * ld + d], X[d * TV + c0 + m], sum);
+            sum *= pw[r];
+            for (int j = 0; j <= min(r, nc - 1); ++j) sum = fmaf(P[r * C + j], V[j * TV + c0 + m], sum);
+          }
 #pragma unroll
         for (int i = 0; i < M; ++i) {
           const int r = ty + 16 * i;

@@ -183,7 +183,9 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
     dk**-0.5; lengths (B,) integers: only the first lengths[b] steps of row b count (held to
     [0, L]), later rows of the output are zero and their inputs are never used; initial_state
     (B, H, dk, dv).  Returns o (B, L, H, dv) in q's dtype [and the state after the last counted step,
-    fp32 (B, H, dk, dv), to continue with this function or :func:`linear_attention_step`].
+    fp32 (B, H, dk, dv), to continue with this function or :func:`linear_attention_step`].  An infinity or NaN
+    among the inputs makes what the recurrence forms from it infinite or NaN (which of them is not defined), and
+    nothing else: no earlier step, other head or row.
 
     dk <= 512, and dv <= 512 for gradients.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
     dv <= 256 too) runs on the tensor cores; everything else on the FP32 pipe.  error_flag: a device int32

@@ -587,6 +587,8 @@ hxm_status hxm_mlstm_gate_epilogue(const hxm_mlstm_gates_args* args, void* strea
 /* from S_(-1) = s0 (zero where NULL); sT (or NULL) receives S_(n-1).  n is     */
 /* lengths[b], held to [0, seqlen], or seqlen where lengths is NULL; out rows  */
 /* n .. seqlen-1 are set to zero and the inputs' rows there are never used.   */
+/* An infinity or NaN among the inputs makes what the recurrence forms from it */
+/* infinite or NaN (which of them is not defined), and nothing else.           */
 /* No reference kernel: the mLSTM recurrence (kernels/tfla/tfla_interface.py:  */
 /* 113-137) with a constant forget gate and without input gate, normalizer.    */
 /* q, k: (b, t, h, dk), v, out: (b, t, h, dv) of the io dtype (bf16 / fp32)   */

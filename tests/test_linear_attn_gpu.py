@@ -361,3 +361,40 @@ def test_captured_training_step(ops, dtype):
     late = torch.autograd.grad([o, sT], eager, ones)
     for a, b, c, d in zip(want, got1, got2, late):
         assert torch.equal(a, b) and torch.equal(a, c) and torch.equal(a, d)
+
+
+@pytest.mark.parametrize("dtype,dims", [(F32, (64, 64)), (BF, (64, 72)), (BF, (128, 128)), (BF, (192, 40)), (BF, (20, 12)), (F32, (300, 33))])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_finite_stay_where_they_belong(ops, dtype, dims, bad):
+    """One element of q (row 0), of k (row 1), of v (row 2) or of dout (row 3) that is not finite, in the middle of a chunk:
+    the recurrence in 64 bits says which outputs, states and gradients are not finite then, and all others keep the
+    bits that they have without it (its tile-mates before it, the other columns, heads and rows among them).  Decays that
+    keep and that forget within a chunk; one long head, cut along time, too."""
+    for L, H, ld in ((300, 3, [-0.01, -0.6, -math.inf]), (1100, 1, [-0.02])):
+        q, k, v, ld, s0 = inputs(5, L, H, *dims, dtype, seed=dims[0], s0=True, ld=torch.tensor(ld, device="cuda"))
+        g = torch.Generator(device="cuda").manual_seed(2)
+        do, dS = torch.randn(v.shape, generator=g, device="cuda").to(dtype), torch.randn(s0.shape, generator=g, device="cuda")
+        run = lambda q, k, v, do: (*ops.linear_attention(q, k, v, ld, initial_state=s0, scale=0.2, return_final_state=True),
+                                   *ops.linear_attention_bwd(q, k, v, ld, do, initial_state=s0, d_final_state=dS, scale=0.2))
+        clean = run(q, k, v, do)
+        x = [t.clone() for t in (q, k, v, do)]
+        for i in range(4):
+            x[i][i, 200, 0, 3] = bad
+        got = run(*x)
+        ref = (*recur(*x[:3], ld, 0.2, None, s0), *grads_ref(*x[:3], ld, 0.2, None, s0, x[3], dS))
+        for i, (a, c, r) in enumerate(zip(got, clean, ref)):
+            fine = torch.isfinite(r)
+            assert torch.equal(torch.where(fine, a, 0), torch.where(fine, c, 0)), i
+            assert not bool((torch.isfinite(a) & ~fine).any()), i
+
+
+@pytest.mark.parametrize("dtype,dims", [(F32, (64, 64)), (BF, (64, 72)), (BF, (192, 40)), (BF, (20, 12))])
+def test_an_infinite_value_leaves_infinite_states(ops, dtype, dims):
+    """The state that an infinite v reaches holds infinities of k's signs, as in the recurrence, not NaN."""
+    q, k, v, ld, s0 = inputs(1, 300, 2, *dims, dtype, seed=4, s0=True, ld=torch.tensor([-0.01, -0.6], device="cuda"))
+    v[0, 200, :, 3] = torch.tensor([float("inf"), -float("inf")], device="cuda")
+    _, sT = ops.linear_attention(q, k, v, ld, initial_state=s0, return_final_state=True)
+    _, ref = recur(q, k, v, ld, 1.0, None, s0)
+    assert torch.equal(sT[..., 3].double(), ref[..., 3]) and bool(torch.isinf(ref[..., 3]).all())
+    keep = [c for c in range(dims[1]) if c != 3]
+    assert bool(torch.isfinite(sT[..., keep]).all())
