@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
   const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2] + e0;
   if (!state_only) {  // rows past the sequence
     const int lo = max(n, u_lo), hi = min(cm.seqlen, u_lo + cm.seg_len);
-    for (int i = tid; i < (hi - lo) * TV; i += 256)
-      if (e0 + i % TV < p.dv) o[(int64_t)(lo + i / TV) * p.so[1] + i % TV] = from_f32<T>(0.f);
+    for (int64_t i = tid; i < (int64_t)(hi - lo) * TV; i += 256)
+      if (e0 + i % TV < p.dv) o[(lo + i / TV) * p.so[1] + i % TV] = from_f32<T>(0.f);
   }
   const bool last_seg = n == 0 ? seg == 0 : (u_lo < n && u_hi == n);
   for (int u0 = u_lo; u0 < u_hi; u0 += C) {

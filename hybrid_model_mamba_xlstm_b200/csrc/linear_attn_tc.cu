@@ -188,9 +188,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
     __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o) + b * p.so[0] + h * p.so[2] + e0;
     if (!state_only) {  // rows past the sequence
       const int lo = max(n, u_lo), hi = min(cm.seqlen, u_lo + cm.seg_len);
-      for (int i = tid; i < (hi - lo) * 8; i += 256)
+      for (int64_t i = tid; i < (int64_t)(hi - lo) * 8; i += 256)
         if (e0 + (i & 7) * 8 < p.dv)
-          *reinterpret_cast<uint4*>(o + (int64_t)(lo + (i >> 3)) * p.so[1] + (i & 7) * 8) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(o + (lo + (i >> 3)) * p.so[1] + (i & 7) * 8) = make_uint4(0, 0, 0, 0);
     }
     const float rf = p.scale * (sep ? (float)exp2(lg2 * (ul - 64)) : 1.f);  // the output row's factor
     auto weigh = [&](int k) -> bool {

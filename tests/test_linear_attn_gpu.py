@@ -398,3 +398,17 @@ def test_an_infinite_value_leaves_infinite_states(ops, dtype, dims):
     assert torch.equal(sT[..., 3].double(), ref[..., 3]) and bool(torch.isinf(ref[..., 3]).all())
     keep = [c for c in range(dims[1]) if c != 3]
     assert bool(torch.isfinite(sT[..., keep]).all())
+
+
+def test_rows_behind_the_lengths_of_a_very_long_batch(ops):
+    """2^25 rows behind the length, of 75 heads (no cut along time), one value column each: 64 columns a block times the
+    rows pass 32 bits.  All of them are zero, and the counted rows are those of a short call."""
+    L, H, n = 2 ** 25 + 70, 75, 5
+    for dtype in (BF, F32):
+        q, k, v, ld, _ = inputs(1, n, H, 1, 1, dtype, seed=1)
+        long = [x[:, :1].expand(1, L, H, 1) for x in (q, k, v)]  # a zero stride: no memory of that length
+        o = ops.linear_attention(*long, ld, lengths=torch.tensor([n], device="cuda"), scale=1.0)
+        want = ops.linear_attention(*(x[:, :1].expand(1, n, H, 1).contiguous() for x in (q, k, v)), ld, scale=1.0)
+        assert torch.equal(o[:, :n], want)
+        assert int(torch.count_nonzero(o[:, n:])) == 0
+        del o
