@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from .. import _lib
 
@@ -65,6 +66,15 @@ def once_only(who):
     """Raises in a backward that is itself being differentiated (create_graph=True): its kernels record nothing."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{who}: its gradient cannot be differentiated again")
+
+
+def no_tangents(who, *tensors):
+    """Raises where a tensor carries a forward-mode tangent: the kernels would drop it without a word."""
+    if _forward_ad._current_level < 0:  # outside of dual_level, torch.func.jvp and the like
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{who}: has no forward-mode derivative")
 
 
 def ptr(t):

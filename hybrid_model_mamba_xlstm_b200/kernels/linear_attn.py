@@ -13,7 +13,7 @@ import math
 import torch
 
 from .. import _lib
-from ._common import dtype_code, on_device, once_only, require_cuda, stream_of
+from ._common import dtype_code, no_tangents, on_device, once_only, require_cuda, stream_of
 
 __all__ = ["linear_attention", "linear_attention_bwd", "linear_attention_step"]
 
@@ -118,6 +118,7 @@ def linear_attention_bwd(q, k, v, log_decay, dout, *, scale=None, lengths=None, 
     ``need_d_initial_state`` (default: with an initial_state).  They are three more runs of the same
     recurrence, dk and dv in reversed time, so dv (the size) may be at most 512 like dk."""
     who = "linear_attention_bwd"
+    no_tangents(who, q, k, v, log_decay, dout, initial_state, d_final_state)
     dev = require_cuda(q, k, v, log_decay, dout, lengths, initial_state, d_final_state, error_flag, who=who)
     if dout.shape != v.shape or dout.dtype != q.dtype:
         raise ValueError(f"{who}: dout must be {tuple(v.shape)} {q.dtype}, got {tuple(dout.shape)} {dout.dtype}")
@@ -194,6 +195,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
     who = "linear_attention"
     if q.dim() != 4:
         raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")
+    no_tangents(who, q, k, v, initial_state, log_decay)
     scale = _scale(who, scale, q.shape[-1])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, initial_state, log_decay)):
         if v.shape[-1] > 512:
@@ -213,6 +215,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
     if given, which shares no memory with q, k or the state).  q, k (B, H, dk), v (B, H, dv): bf16 or fp32.
     Without gradients."""
     who = "linear_attention_step"
+    no_tangents(who, q, k, v, log_decay, state)
     dev = require_cuda(q, k, v, log_decay, state, out, who=who)
     if q.dim() != 3:
         raise ValueError(f"{who}: q must be (B, H, dk), got {tuple(q.shape)}")

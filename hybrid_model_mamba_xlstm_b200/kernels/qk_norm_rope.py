@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from ._common import dtype_code, on_device, once_only, require_cuda, stream_of
+from ._common import dtype_code, no_tangents, on_device, once_only, require_cuda, stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_bwd"]
 
@@ -92,6 +92,7 @@ def qk_norm_rope_bwd(q, k, q_weight, k_weight, dq_out, dk_out, positions=None, *
     dk_weight): the first two in q's dtype, the weights' fp32 (None for a weight that is None, or without
     ``weight_grads``)."""
     who = "qk_norm_rope_bwd"
+    no_tangents(who, q, k, q_weight, k_weight, dq_out, dk_out)
     dev = require_cuda(q, k, q_weight, k_weight, dq_out, dk_out, positions, who=who)
     if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.dtype != q.dtype or dk_out.dtype != k.dtype:
         raise ValueError(f"{who}: the gradients must match q and k")
@@ -138,6 +139,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, positions=None, *, rope_bas
     one projection's output); weights (d,) or None (ones); positions (B, L) or (L,) integers, the angles
     formed in 64 bits.  d <= 1024; eps at least 0 (0: a row of zeros gives NaN, as the formula does).  Returns
     the two results, dense, in q's dtype."""
+    no_tangents("qk_norm_rope", q, k, q_weight, k_weight)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         return QkNormRopeFunction.apply(q, k, q_weight, k_weight, positions, rope_base, rotary_dim, interleaved, eps)

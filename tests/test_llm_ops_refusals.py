@@ -147,3 +147,22 @@ def test_norms_eps(eps):
     b.fwd = a
     got, said = call("hxm_qk_norm_rope_bwd", b)
     assert got == _lib.HXM_EBADARG and "eps" in said
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost silently: none of the operators has forward-mode derivatives."""
+    x, ld = torch.zeros(1, 4, 2, 8), torch.zeros(2)
+    calls = [lambda t: kernels.linear_attention(t, x, x, ld), lambda t: kernels.linear_attention(x, x, t, ld),
+             lambda t: kernels.linear_attention(x, x, x, ld, initial_state=t.new_zeros(1, 2, 8, 8) + t[0, 0, 0, 0]),
+             lambda t: kernels.linear_attention(x, x, x, t[0, 0, :, 0]),
+             lambda t: kernels.linear_attention_step(x[0], t[0], x[0], ld, torch.zeros(4, 2, 8, 8)),
+             lambda t: kernels.qk_norm_rope(t, x), lambda t: kernels.qk_norm_rope(x, x, None, t[0, 0, 0]),
+             lambda t: kernels.linear_attention_bwd(x, x, x, ld, t), lambda t: kernels.qk_norm_rope_bwd(x, x, None, None, x, t)]
+    for go in calls:
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                go(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+            with pytest.raises(RuntimeError, match="CUDA device"):  # no tangent: as ever
+                go(x)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda t: go(t), (x,), (torch.ones_like(x),))
