@@ -286,7 +286,8 @@ static int generic_tile(int dk) { return generic_smem(64, 64, padded_dk(dk)) + s
 template <typename T, int C>
 static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int dv, bool state_only, cudaStream_t st) {
   const size_t smem = generic_smem(C, C, dkp);
-  HXM_CUDA_TRY(cudaFuncSetAttribute(generic_kernel<T, C, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const hxm_status s = allow_shared_memory<generic_kernel<T, C, C>>();
+  if (s != HXM_OK) return s;
   const dim3 grid((unsigned)((dv + C - 1) / C * gp.c.nseg), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
   generic_kernel<T, C, C><<<grid, 256, smem, st>>>(gp, dkp, state_only ? 1 : 0);
   return check_launch("hxm_linear_attn");

@@ -696,7 +696,8 @@ static hxm_status launch_dk(TcParams& t, int np, int tiles, bool state_only, cud
     return cudaFuncGetAttributes(&at, tc_kernel<DK>) == cudaSuccess ? at.numRegs : -1;
   }();
   HXM_REQUIRE_SUPPORTED(regs == kRegsLaunch, "hxm_linear_attn: built with %d registers a thread, not %d", regs, kRegsLaunch);
-  HXM_CUDA_TRY(cudaFuncSetAttribute(tc_kernel<DK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const hxm_status s = allow_shared_memory<tc_kernel<DK>>();
+  if (s != HXM_OK) return s;
   const dim3 grid((unsigned)(tiles * t.c.nseg), (unsigned)t.c.heads, (unsigned)(t.c.batch * np));
   tc_kernel<DK><<<grid, kThreadsTc, smem, st>>>(t, tiles, state_only ? 1 : 0);
   return check_launch("hxm_linear_attn");

@@ -423,7 +423,8 @@ static hxm_status launch(Params& p, cudaStream_t st) {
   const int64_t tokens = (int64_t)p.batch * p.seqlen;
   const unsigned grid = BWD ? (unsigned)(p.blocks = kBwdBlocksRow) : (unsigned)(tokens < 16 * kSMs ? tokens : 16 * kSMs);
   const size_t smem = (size_t)(p.rotary / 2) * sizeof(float2) + sizeof(float) * p.dim * (kThreads / 32) * (BWD ? 4 : 2);
-  HXM_CUDA_TRY(cudaFuncSetAttribute(row_kernel<T, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const hxm_status s = allow_shared_memory<row_kernel<T, BWD>>();
+  if (s != HXM_OK) return s;
   row_kernel<T, BWD><<<grid, kThreads, smem, st>>>(p);
   return check_launch("hxm_qk_norm_rope");
 }

@@ -1072,8 +1072,8 @@ static hxm_status launch(Params p, int rows, cudaStream_t st) {
   while (cl < 8 && (int64_t)rows * cl * 2 <= 2 * 148 && p.vocab / cl > 4 * kThreads) cl *= 2;
   p.slice = ((p.vocab + cl - 1) / cl + 7) / 8 * 8;
   const size_t smem = kRegion + (size_t)(p.slice + 8) * sizeof(K);  // 8: kernel's pad
-  HXM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  HXM_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  const hxm_status s = allow_shared_memory<sample_kernel<T>, true>();
+  if (s != HXM_OK) return s;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * cl));
   cfg.blockDim = dim3(kThreads);

@@ -313,3 +313,45 @@ def test_norms_refuse_an_eps_that_is_none(ops):
             ops.qk_norm_rope(q, q, w, w, eps=eps)
         with pytest.raises(ValueError, match="eps"):
             ops.qk_norm_rope_bwd(q, q, w, w, q, q, eps=eps)
+
+
+def test_threads_with_calls_of_other_sizes(ops):
+    """Threads whose calls of one kernel need different amounts of shared memory: each result is the one of a call alone
+    (no call is refused because another thread's needs less)."""
+    def attn(dk, L):
+        q, k, v, ld, s0 = inputs(1, L, 2, dk, 20, F32, seed=dk)
+        return lambda: ops.linear_attention(q, k, v, ld)
+
+    def norms(d):
+        x = torch.randn(1, 3, 2, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d))
+        w = torch.ones(d, device="cuda")
+        return lambda: torch.cat([t.flatten() for t in ops.qk_norm_rope_bwd(x, x, w, w, x, x)])
+
+    def tokens(V):
+        x = torch.randn(2, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+        u = torch.tensor([0.3, 0.8], device="cuda")
+        return lambda: ops.sample_tokens(x, u, top_k=20)
+
+    kinds = [[attn(20, 40), attn(130, 40), attn(250, 40)], [norms(33), norms(501), norms(1001)], [tokens(300), tokens(50000), tokens(260000)]]
+    for calls in kinds:
+        want = [c().clone() for c in calls]
+        torch.cuda.synchronize()
+        wrong, errors = [], []
+
+        def work(i):
+            try:
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    for _ in range(300):
+                        got = calls[i % 3]()
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(got, want[i % 3]):
+                        wrong.append(i)
+            except Exception as e:
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(9)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors and not wrong, (errors[:1], wrong)
