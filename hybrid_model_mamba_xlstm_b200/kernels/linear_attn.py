@@ -78,7 +78,7 @@ def _fill(who, q, k, v, log_decay, scale, lengths, s0, out, sT, error_flag, wait
         if lengths.shape != (bsz,) or lengths.is_floating_point() or lengths.dtype == torch.bool:
             raise ValueError(f"{who}: lengths must be ({bsz},) integers")
         if lengths.dtype != torch.int32:
-            lengths = lengths.clamp(0, L).int()
+            lengths = lengths.long().clamp(0, L).int()  # widened first: L may be beyond the type's range
         lengths = lengths.contiguous()
     if s0 is not None:
         if s0.shape != (bsz, nh, dk, v.shape[-1]):

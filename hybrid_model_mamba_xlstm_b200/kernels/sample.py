@@ -48,7 +48,7 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=None, top_p=None, 
                 if name == "top_k":
                     if x.is_floating_point() or x.dtype == torch.bool:
                         raise TypeError(f"{who}: top_k must be integers, got {x.dtype}")
-                    x = x if x.dtype == torch.int32 else x.clamp(0, vocab).int()
+                    x = x if x.dtype == torch.int32 else x.long().clamp(0, vocab).int()  # the type may not hold vocab
                 keep.append((x if name == "top_k" else x.float()).contiguous())
                 return off, keep[-1].data_ptr()
             if x is None:

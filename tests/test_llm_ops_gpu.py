@@ -355,3 +355,19 @@ def test_threads_with_calls_of_other_sizes(ops):
         for t in threads:
             t.join()
         assert not errors and not wrong, (errors[:1], wrong)
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_integers_of_every_type(ops, kind):
+    """lengths, per-row top_k and positions in a type that does not reach the sequence's or the vocabulary's size."""
+    n = torch.tensor([0, 1, 100], device="cuda")
+    q, k, v, ld, _ = inputs(3, 777, 2, 16, 16, F32, seed=1)
+    assert torch.equal(ops.linear_attention(q, k, v, ld, lengths=n.to(kind)), ops.linear_attention(q, k, v, ld, lengths=n.int()))
+    x, u = torch.randn(3, 50304, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)), torch.tensor([0.1, 0.5, 0.9], device="cuda")
+    assert torch.equal(ops.sample_tokens(x, u, top_k=n.to(kind)), ops.sample_tokens(x, u, top_k=n.int()))
+    a, b = ops.qk_norm_rope(q[:, :3], k[:, :3], None, None, n.to(kind)), ops.qk_norm_rope(q[:, :3], k[:, :3], None, None, n)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+    if kind not in (torch.uint8,):
+        m = torch.tensor([-3, 5, 127], device="cuda")
+        assert torch.equal(ops.linear_attention(q, k, v, ld, lengths=m.to(kind)), ops.linear_attention(q, k, v, ld, lengths=m.clamp(min=0)))
+        assert torch.equal(ops.sample_tokens(x, u, top_k=m.to(kind)), ops.sample_tokens(x, u, top_k=m.clamp(min=0)))
