@@ -78,7 +78,8 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
   const Common& cm = gp.c;
   const int b = blockIdx.z % cm.batch;
   const Problem& p = gp.p[blockIdx.z / cm.batch];
-  const int h = blockIdx.y, seg = blockIdx.x % cm.nseg, e0 = (blockIdx.x / cm.nseg) * TV;
+  const int segs = cm.nseg - state_only;  // the last one's sum is nobody's entering state
+  const int h = blockIdx.y, seg = blockIdx.x % segs, e0 = (blockIdx.x / segs) * TV;
   if (e0 >= p.dv) return;
   const int ld = dkp + 4;  // row pitch of Q, K
   extern __shared__ __align__(16) float sh[];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
   }
   __syncthreads();
   if (state_only) {
-    if (seg < cm.nseg - 1 && u_lo < n)
+    if (u_lo < n)
       for (int i = tid; i < dkp * TV; i += 256) {
         const int d = i / TV, e = e0 + i % TV;
         if (d < p.dk && e < p.dv) p.ws[((((int64_t)b * cm.heads + h) * (cm.nseg - 1) + seg) * p.dk + d) * p.dv + e] = X[i];
@@ -288,7 +289,7 @@ static hxm_status launch_generic_c(const GenericParams& gp, int np, int dkp, int
   const size_t smem = generic_smem(C, C, dkp);
   const hxm_status s = allow_shared_memory<generic_kernel<T, C, C>>();
   if (s != HXM_OK) return s;
-  const dim3 grid((unsigned)((dv + C - 1) / C * gp.c.nseg), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
+  const dim3 grid((unsigned)((dv + C - 1) / C * (gp.c.nseg - (state_only ? 1 : 0))), (unsigned)gp.c.heads, (unsigned)(gp.c.batch * np));
   generic_kernel<T, C, C><<<grid, 256, smem, st>>>(gp, dkp, state_only ? 1 : 0);
   return check_launch("hxm_linear_attn");
 }

@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       int64_t sd = p.dv, se = 1;
       float f = 1.f;
       if (state_only) {
-        if (seg < cm.nseg - 1 && u_lo < n)
+        if (u_lo < n)
           dst = p.ws + (((int64_t)b * cm.heads + h) * (cm.nseg - 1) + seg) * p.dk * p.dv;
       } else if (p.sT && (n == 0 ? seg == 0 : u_lo < n && u_hi == n)) {
         dst = p.sT + b * p.sTs[0] + h * p.sTs[1];
@@ -698,7 +698,8 @@ static hxm_status launch_dk(TcParams& t, int np, int tiles, bool state_only, cud
   HXM_REQUIRE_SUPPORTED(regs == kRegsLaunch, "hxm_linear_attn: built with %d registers a thread, not %d", regs, kRegsLaunch);
   const hxm_status s = allow_shared_memory<tc_kernel<DK>>();
   if (s != HXM_OK) return s;
-  const dim3 grid((unsigned)(tiles * t.c.nseg), (unsigned)t.c.heads, (unsigned)(t.c.batch * np));
+  // the last segment's sum is nobody's entering state
+  const dim3 grid((unsigned)(tiles * (t.c.nseg - (state_only ? 1 : 0))), (unsigned)t.c.heads, (unsigned)(t.c.batch * np));
   tc_kernel<DK><<<grid, kThreadsTc, smem, st>>>(t, tiles, state_only ? 1 : 0);
   return check_launch("hxm_linear_attn");
 }
