@@ -412,3 +412,24 @@ def test_rows_behind_the_lengths_of_a_very_long_batch(ops):
         assert torch.equal(o[:, :n], want)
         assert int(torch.count_nonzero(o[:, n:])) == 0
         del o
+
+
+@pytest.mark.parametrize("dims", [(1, 257, 2, 128, 64), (2, 300, 2, 64, 72), (1, 300, 1, 256, 64), (1, 2600, 1, 128, 64)])
+def test_bf16_states_to_32_bits(ops, dims):
+    """The last state and the first state's gradient of bf16 runs.  k is bf16 as it is, and a weighted v goes into the
+    products in three bf16 parts, whose half steps leave at most 2^-8, 2^-16 and 2^-24 of it behind the first, the
+    second and the third: two parts would leave some 2^-19 of the state's norm.  With three a term carries the roundings
+    of its weight and of its product with v, the parts' rest, and the roundings of the factors of the chunks behind it
+    that still count (two): 5 2^-24.  A chunk's sum is 8 steps of 16 terms for each of 3 parts, 24 additions in fp32
+    whose errors are independent: sqrt(24) 2^-24 of the norm."""
+    B, L, H, dk, dv = dims
+    ld = torch.tensor([-0.03, -0.002], device="cuda")[-H:]  # (powers of 1/2 would leave v in one part)
+    q, k, v, ld, s0 = inputs(B, L, H, dk, dv, BF, seed=L, s0=True, ld=ld)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    do, dS = torch.randn(v.shape, generator=g, device="cuda").to(BF), torch.randn(s0.shape, generator=g, device="cuda")
+    _, sT = ops.linear_attention(q, k, v, ld, initial_state=s0, scale=0.3, return_final_state=True)
+    _, rS = recur(q, k, v, ld, 0.3, None, s0)
+    ds = ops.linear_attention_bwd(q, k, v, ld, do, initial_state=s0, d_final_state=dS, scale=0.3)[3]
+    rd = grads_ref(q, k, v, ld, 0.3, None, s0, do, dS)[3]
+    for a, b in ((sT, rS), (ds, rd)):
+        assert float((a.double() - b).norm() / b.norm()) <= (5 + 24 ** 0.5) * 2.0 ** -24

@@ -234,3 +234,22 @@ def test_streams_and_graph(sample):
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_settings_of_rows_in_other_types(sample):
+    """Per-row settings count as fp32 and as whole numbers whatever their types; top_k below 1 keeps all, temperatures
+    not above 0 are greedy."""
+    B, V = 64, 3001
+    logits, u = make(B, V, torch.bfloat16, seed=4)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    pick = lambda vals, kind: torch.tensor(vals, device="cuda", dtype=kind)[torch.randint(0, len(vals), (B,), generator=g, device="cuda")]
+    T, K = pick([0.0, 0.5, 1.0, -1.0], torch.float32), pick([-2, 0, 1, 13, 5000], torch.int32)
+    P, M = pick([0.125, 0.875, 1.0], torch.float32), pick([0.0, 0.0625], torch.float32)
+    want = check(sample, logits, u, T, K.clamp(min=0), P, M)
+    for t, k, p, m in ((T, K, P, M), (T.double(), K.long(), P.double(), M.double()), (T.half(), K.short(), P.half(), M.bfloat16()),
+                       (T, K, P, 0.0)):
+        if torch.is_tensor(m):
+            assert torch.equal(want, sample(logits, u, temperature=t, top_k=k, top_p=p, min_p=m))
+        else:
+            assert torch.equal(sample(logits, u, temperature=t, top_k=k, top_p=p, min_p=torch.zeros_like(M)),
+                               sample(logits, u, temperature=t, top_k=k, top_p=p))
