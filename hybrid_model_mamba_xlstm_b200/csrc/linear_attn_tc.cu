@@ -61,8 +61,8 @@ struct Layout {
   static constexpr int kVs = kSnap + DK * 128;    // the scaled V's parts
   static constexpr int kPw = kVs + kParts * kPanel;  // float[132]: g^0 .. g^128
   static constexpr int kCf = kPw + 132 * 4;       // float[128]: g^(64 - step) by tile row
-  static constexpr int kBar = kCf + 128 * 4;      // 19 mbarriers
-  static constexpr int kSlot = kBar + 19 * 8;
+  static constexpr int kBar = kCf + 128 * 4;      // 20 mbarriers
+  static constexpr int kSlot = kBar + 20 * 8;
   static constexpr int kBytes = kSlot + 16;
   // TMEM columns: two S / P; two O (or O1, O2); U: the first two parts of the scaled V side by side
   // (dk <= 128), or one sum per 128 rows of X
@@ -117,12 +117,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
   uint64_t* p_ready = full + 6;   // [2] group A: P in TMEM
   uint64_t* o_ready = full + 8;   // [2] MMA: O
   uint64_t* o_free = full + 10;   // [2] group A: O read
-  uint64_t* x_ready = full + 12;  // group B: bf16 X written
-  uint64_t* v_ready = full + 13;  // group B: scaled V written, U of the chunk before read
-  uint64_t* u_ready = full + 14;  // MMA: U
-  uint64_t* qs_done = full + 15;  // MMA: bf16 X read
-  uint64_t* fin = full + 16;
-  uint64_t* v_checked = full + 17;  // [2] check warps (a chunk ahead at most): V and its parts fit for the products
+  uint64_t* v_ready = full + 12;  // [2] group B: scaled V written, U of the chunk before read
+  uint64_t* v_checked = full + 14;  // [2] check warps (a chunk ahead at most): V and its parts fit for the products
+  uint64_t* x_ready = full + 16;  // group B: bf16 X written
+  uint64_t* u_ready = full + 17;  // MMA: U
+  uint64_t* qs_done = full + 18;  // MMA: bf16 X read
+  uint64_t* fin = full + 19;
   uint32_t* slot = reinterpret_cast<uint32_t*>(sm + Lt::kSlot);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Lt::kSlot + 4);
   volatile int* not_finite = reinterpret_cast<volatile int*>(sm + Lt::kSlot + 8);  // check warps: met such a v
@@ -147,10 +147,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       tc::mbar_init(p_ready + i, 8);
       tc::mbar_init(o_ready + i, 1);
       tc::mbar_init(o_free + i, 8);
+      tc::mbar_init(v_ready + i, kWarpsB);
       tc::mbar_init(v_checked + i, 2);
     }
     tc::mbar_init(x_ready, kWarpsB);
-    tc::mbar_init(v_ready, kWarpsB);
     tc::mbar_init(u_ready, 1);
     tc::mbar_init(qs_done, 1);
     tc::mbar_init(fin, 1);
@@ -424,17 +424,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
           *reinterpret_cast<uint4*>(sm + Lt::kVs + part * kPanel + tc::sw128_offset(row, cb + 8 * q)) =
               make_uint4(vp[part][4 * q], vp[part][4 * q + 1], vp[part][4 * q + 2], vp[part][4 * q + 3]);
     };
-    auto v_done = [&]() {
+    auto v_done = [&](int k) {
       tc::fence_async_smem();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(v_ready);
+      if (lane == 0) tc::mbar_arrive(v_ready + (k & 1));
     };
     snapshot();
     bool ok = nch == 0 || scale_v(0);
     if (ok && nch) {
       store_v();
-      v_done();
+      v_done(0);
     }
 #pragma unroll 1
     for (int k = 0; ok && k < nch; ++k) {
@@ -454,13 +454,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
         for (int j = 0; j < 16; ++j) x[j] = kNB == 2 || i == 0 ? fmaf(f, x[j], u[j]) : x[j] + u[j];
       }
       if (!more) break;
-      if (kStages == 2) v_done();
+      if (kStages == 2) v_done(k + 1);
       if (!state_only && !(ok = wait(qs_done, k))) break;
       snapshot();
       if (kStages == 1) {
         if (!(ok = scale_v(k + 1))) break;
         store_v();
-        v_done();
+        v_done(k + 1);
       }
     }
     if (ok) {
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       for (int k = 0; ok && k < nch; ++k) {
         const int st = k % kStages;
         if (state_only && !(ok = w8(full + st, k / kStages))) break;
-        if (!(ok = w8(v_ready, k) && w8(v_checked + (k & 1), k >> 1))) break;
+        if (!(ok = w8(v_ready + (k & 1), k >> 1) && w8(v_checked + (k & 1), k >> 1))) break;
         tc::tc_fence_after();
         issue_u(k);
         if (state_only) {
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
         most = __vmaxu2(__vmaxu2(most, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
       }
       if (__any_sync(0xffffffffu, (most & 0xffffu) >= 0x7f80u || (most >> 16) >= 0x7f80u)) {
-        if (!wait(v_ready, k)) break;  // group B has read V, and put zeros into its rows past the end
+        if (!wait(v_ready + (k & 1), k >> 1)) break;  // group B has read V, and put zeros into its rows past the end
 #pragma unroll 1
         for (int w = 0; w < kPanel / 256; ++w) {  // word w of this lane's
           const int i = (w >> 2) * 1024 + (w & 3) * 4;

@@ -433,3 +433,23 @@ def test_bf16_states_to_32_bits(ops, dims):
     rd = grads_ref(q, k, v, ld, 0.3, None, s0, do, dS)[3]
     for a, b in ((sT, rS), (ds, rd)):
         assert float((a.double() - b).norm() / b.norm()) <= (5 + 24 ** 0.5) * 2.0 ** -24
+
+
+def test_repeats_with_values_behind_the_lengths(ops):
+    """NaN and infinities behind the ends of rows of one, two and three chunks, many times over while other work keeps the
+    clocks apart: the same bits as with zeros there."""
+    lengths = torch.tensor([1, 127, 129, 130, 200, 257, 299], device="cuda")
+    behind = torch.arange(300, device="cuda")[None, :] >= lengths[:, None]
+    other = torch.randn(2048, 2048, device="cuda")
+    for dk in (64, 192):
+        q, k, v, ld, s0 = inputs(7, 300, 2, dk, 72, BF, seed=6, s0=True)
+        zeros, bad = [x.clone() for x in (q, k, v)], [x.clone() for x in (q, k, v)]
+        for x, y, value in zip(zeros, bad, (float("nan"), float("inf"), float("nan"))):
+            x[behind], y[behind] = 0, value
+        call = lambda x: (*ops.linear_attention(*x, ld, lengths=lengths, initial_state=s0, return_final_state=True),
+                          *ops.linear_attention_bwd(*x, ld, x[2], lengths=lengths, initial_state=s0))
+        want = call(zeros)
+        for i in range(100):
+            if i % 2:
+                other @ other
+            assert all(torch.equal(a, b) for a, b in zip(call(bad), want)), i
