@@ -206,20 +206,11 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
             for (int i = 0; i < M; ++i) fma_row(acc[i], m == 0 ? a[i].x : m == 1 ? a[i].y : m == 2 ? a[i].z : a[i].w, x);
           }
         }
-        // An infinity or NaN in V reached the rows before it too (their weights are 0, and 0 * inf is NaN): sums that are
-        // not finite are formed again, from the steps up to their row alone.
+        float2 odd = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < M; ++i)
 #pragma unroll
-          for (int m = 0; m < N; ++m) {
-            float& sum = m & 1 ? acc[i].v[m / 2].y : acc[i].v[m / 2].x;
-            if (sum - sum == 0.f) continue;
-            const int r = ty + 16 * i;
-            sum = 0.f;
-            for (int d = 0; d < dkp; ++d) sum = fmaf(Q[r * ld + d], X[d * TV + c0 + m], sum);
-            sum *= pw[r];
-            for (int j = 0; j <= min(r, nc - 1); ++j) sum = fmaf(P[r * C + j], V[j * TV + c0 + m], sum);
-          }
+          for (int m = 0; m < N / 2; ++m) odd = __ffma2_rn(acc[i].v[m], make_float2(0.f, 0.f), odd);
 #pragma unroll
         for (int i = 0; i < M; ++i) {
           const int r = ty + 16 * i;
@@ -229,6 +220,22 @@ __global__ void __launch_bounds__(256, 1) generic_kernel(const __grid_constant__
           for (int m = 0; m < N / 2; ++m) {
             if (e0 + c0 + 2 * m < p.dv) row[2 * m] = from_f32<T>(p.scale * acc[i].v[m].x);
             if (e0 + c0 + 2 * m + 1 < p.dv) row[2 * m + 1] = from_f32<T>(p.scale * acc[i].v[m].y);
+          }
+        }
+        // An infinity or NaN in V reached the rows before it too (their weights are 0, and 0 * inf is NaN): a thread
+        // with a sum that is not finite forms all of its sums again, each from the steps up to its row alone.
+        if (odd.x + odd.y != 0.f) {
+#pragma unroll 1
+          for (int i = 0; i < M * N; ++i) {
+            const int r = ty + 16 * (i / N), c = c0 + i % N;
+            if (r >= nc || e0 + c >= p.dv) continue;
+            float sum = 0.f;
+#pragma unroll 1
+            for (int d = 0; d < dkp; ++d) sum = fmaf(Q[r * ld + d], X[d * TV + c], sum);
+            sum *= pw[r];
+#pragma unroll 1
+            for (int j = 0; j <= r; ++j) sum = fmaf(P[r * C + j], V[j * TV + c], sum);
+            o[(t0 + (int64_t)r * dt) * p.so[1] + c] = from_f32<T>(p.scale * sum);
           }
         }
       }

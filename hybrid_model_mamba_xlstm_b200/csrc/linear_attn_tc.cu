@@ -17,11 +17,10 @@
 //
 // Work is cut by role, so that the tensor core always has something queued while one chunk's
 // element-wise work runs: warps 0-7 (group A) turn S into P and write the output; warps 8-23 (group B)
-// scale V, keep X and write its bf16 copy; warp 24 issues the MMAs, warp 25 the TMA loads; warps 26 and
-// 27 look for values in V that are not finite.  S, O and the operand stages are double-buffered
-// (dk <= 128), so S of the next chunk is made while this one's P is, and group B has the next chunk's
-// scaled V in registers when U of this one is done: the only chain from chunk to chunk is
-// U -> X -> bf16(X).
+// scale V, keep X and write its bf16 copy; warp 24 issues the MMAs, warp 25 the TMA loads.  S, O and the
+// operand stages are double-buffered (dk <= 128), so S of the next chunk is made while this one's P is,
+// and group B has the next chunk's scaled V in registers when U of this one is done: the only chain
+// from chunk to chunk is U -> X -> bf16(X).
 // Reversed time (the gradients) only mirrors a chunk: row r of a tile is step 127 - r, which flips the
 // causal mask and the exponents' sign.
 #include "capi_internal.h"
@@ -36,7 +35,8 @@ constexpr int kC = 128;    // steps per chunk
 constexpr int kDV = 64;    // value columns per CTA
 constexpr int kParts = 3;  // bf16 parts of a scaled V value: 2^-24 left over
 constexpr int kPanel = 16384;  // 128 rows x 128 bytes
-// Two warpgroups of group A, four of B, and one for the MMA, TMA and check warps.
+// Two warpgroups of group A, four of B, and one for the MMA and TMA warps (its other two warps only
+// give up their registers).
 constexpr int kThreadsTc = 7 * 128;
 constexpr int kWarpsB = 16;
 // Registers a thread: the launch gives 72 to all; the last warpgroup goes down to 40 and group A,
@@ -61,8 +61,8 @@ struct Layout {
   static constexpr int kVs = kSnap + DK * 128;    // the scaled V's parts
   static constexpr int kPw = kVs + kParts * kPanel;  // float[132]: g^0 .. g^128
   static constexpr int kCf = kPw + 132 * 4;       // float[128]: g^(64 - step) by tile row
-  static constexpr int kBar = kCf + 128 * 4;      // 20 mbarriers
-  static constexpr int kSlot = kBar + 20 * 8;
+  static constexpr int kBar = kCf + 128 * 4;      // 18 mbarriers
+  static constexpr int kSlot = kBar + 18 * 8;
   static constexpr int kBytes = kSlot + 16;
   // TMEM columns: two S / P; two O (or O1, O2); U: the first two parts of the scaled V side by side
   // (dk <= 128), or one sum per 128 rows of X
@@ -117,15 +117,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
   uint64_t* p_ready = full + 6;   // [2] group A: P in TMEM
   uint64_t* o_ready = full + 8;   // [2] MMA: O
   uint64_t* o_free = full + 10;   // [2] group A: O read
-  uint64_t* v_ready = full + 12;  // [2] group B: scaled V written, U of the chunk before read
-  uint64_t* v_checked = full + 14;  // [2] check warps (a chunk ahead at most): V and its parts fit for the products
-  uint64_t* x_ready = full + 16;  // group B: bf16 X written
-  uint64_t* u_ready = full + 17;  // MMA: U
-  uint64_t* qs_done = full + 18;  // MMA: bf16 X read
-  uint64_t* fin = full + 19;
+  uint64_t* x_ready = full + 12;  // group B: bf16 X written
+  uint64_t* v_ready = full + 13;  // group B: scaled V written, U of the chunk before read
+  uint64_t* u_ready = full + 14;  // MMA: U
+  uint64_t* qs_done = full + 15;  // MMA: bf16 X read
+  uint64_t* fin = full + 16;
   uint32_t* slot = reinterpret_cast<uint32_t*>(sm + Lt::kSlot);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + Lt::kSlot + 4);
-  volatile int* not_finite = reinterpret_cast<volatile int*>(sm + Lt::kSlot + 8);  // check warps: met such a v
+  volatile int* not_finite = reinterpret_cast<volatile int*>(sm + Lt::kSlot + 8);  // group B: met such a v
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wq = warp & 3, hf = (warp >> 2) & 1;  // TMEM lane quarter, column half
@@ -147,10 +146,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       tc::mbar_init(p_ready + i, 8);
       tc::mbar_init(o_ready + i, 1);
       tc::mbar_init(o_free + i, 8);
-      tc::mbar_init(v_ready + i, kWarpsB);
-      tc::mbar_init(v_checked + i, 2);
     }
     tc::mbar_init(x_ready, kWarpsB);
+    tc::mbar_init(v_ready, kWarpsB);
     tc::mbar_init(u_ready, 1);
     tc::mbar_init(qs_done, 1);
     tc::mbar_init(fin, 1);
@@ -245,9 +243,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       if (lane == 0) tc::mbar_arrive(p_ready + buf);
       return true;
     };
-    // Zeros stand in V for the values that are not finite (see the check warps): these make the outputs of their own
-    // and of the later steps NaN.  From the chunk on in which the first one was met; rare, so all v of the chunk up to
-    // this row's step are simply read again.
+    // Zeros stand in V for the values that are not finite (see store_v): these make the outputs of their own and of the
+    // later steps NaN.  From the chunk on in which the first one was met; rare, so all v of the chunk up to this
+    // row's step are simply read again.
     auto not_finite_rows = [&](int k, float (&a)[32]) {
       const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.v) + b * p.sv[0] + h * p.sv[2] + e0 + ch;
 #pragma unroll 1
@@ -416,25 +414,43 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       }
       return true;
     };
-    auto store_v = [&]() {
+    auto store_v = [&](int k) {
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           *reinterpret_cast<uint4*>(sm + Lt::kVs + part * kPanel + tc::sw128_offset(row, cb + 8 * q)) =
               make_uint4(vp[part][4 * q], vp[part][4 * q + 1], vp[part][4 * q + 2], vp[part][4 * q + 3]);
+      // An infinity or NaN in V would go with P V to the steps before it (their weights are 0, and 0 * inf is NaN).  So it
+      // leaves V as a zero, and group A brings it to the outputs that it belongs to.  For the state it stays in the
+      // first part, and the others are 0 (inf - inf is NaN).  (Looked for here, where it costs no spills for dk <= 128:
+      // 8 x 2048 x 16 heads of 128 101.1 -> 103.0 us, 4 x 2048 x 16 of 256 101 -> 105.6; by the two idle warps 108.)
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = __vmaxu2(most, vp[0][j] & 0x7fff7fffu);
+      if (__any_sync(0xffffffffu, (most & 0xffffu) >= 0x7f80u || (most >> 16) >= 0x7f80u)) {
+        *not_finite = 1;
+#pragma unroll 1
+        for (int c = 0; c < 16; c += 2) {
+          const uint32_t at = tc::sw128_offset(row, cb + (c & 8)) + 2 * (c & 7);
+          uint32_t* x = reinterpret_cast<uint32_t*>(sm + (k % kStages) * Lt::kStage + Lt::kV + at);
+          const uint32_t keep = ((*x & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((*x & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
+          *x &= keep;
+          for (int part = 1; part < kParts; ++part) *reinterpret_cast<uint32_t*>(sm + Lt::kVs + part * kPanel + at) &= keep;
+        }
+      }
     };
-    auto v_done = [&](int k) {
+    auto v_done = [&]() {
       tc::fence_async_smem();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(v_ready + (k & 1));
+      if (lane == 0) tc::mbar_arrive(v_ready);
     };
     snapshot();
     bool ok = nch == 0 || scale_v(0);
     if (ok && nch) {
-      store_v();
-      v_done(0);
+      store_v(0);
+      v_done();
     }
 #pragma unroll 1
     for (int k = 0; ok && k < nch; ++k) {
@@ -443,7 +459,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       if (!(ok = wait(u_ready, k))) break;
       tc::tc_fence_after();
       const float f = pw[end_of(k)];
-      if (kStages == 2 && more) store_v();
+      if (kStages == 2 && more) store_v(k + 1);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {  // the parts' two sums (dk <= 128), or the two halves of X
         float u[16];
@@ -454,13 +470,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
         for (int j = 0; j < 16; ++j) x[j] = kNB == 2 || i == 0 ? fmaf(f, x[j], u[j]) : x[j] + u[j];
       }
       if (!more) break;
-      if (kStages == 2) v_done(k + 1);
+      if (kStages == 2) v_done();
       if (!state_only && !(ok = wait(qs_done, k))) break;
       snapshot();
       if (kStages == 1) {
         if (!(ok = scale_v(k + 1))) break;
-        store_v();
-        v_done(k + 1);
+        store_v(k + 1);
+        v_done();
       }
     }
     if (ok) {
@@ -556,7 +572,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
       for (int k = 0; ok && k < nch; ++k) {
         const int st = k % kStages;
         if (state_only && !(ok = w8(full + st, k / kStages))) break;
-        if (!(ok = w8(v_ready + (k & 1), k >> 1) && w8(v_checked + (k & 1), k >> 1))) break;
+        if (!(ok = w8(v_ready, k))) break;
         tc::tc_fence_after();
         issue_u(k);
         if (state_only) {
@@ -631,42 +647,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tc_kernel(const __grid_constant
         tc::mbar_wait(full + k % kStages, (k / kStages) & 1, &none, 20000000ll);
     }
     __syncwarp();
-  } else {
-    // ======================= check of V (two warps) =======================
-    // An infinity or NaN in V would go with P V to the steps before it (their weights are 0, and 0 * inf is NaN).  So it
-    // leaves V as a zero, and group A brings it to the outputs that it belongs to.  For the state it stays in the first
-    // part of the scaled V, and the other parts are 0 (inf - inf is NaN).
-    const int off = ((warp & 1) * 32 + lane) * 16;
-#pragma unroll 1
-    for (int k = 0; k < nch; ++k) {
-      const int st = k % kStages;
-      unsigned char* v = sm + st * Lt::kStage + Lt::kV + off;
-      if (!wait(full + st, k / kStages)) break;
-      uint32_t most = 0;
-#pragma unroll 4
-      for (int i = 0; i < kPanel; i += 1024) {
-        const uint4 x = *reinterpret_cast<const uint4*>(v + i);
-        most = __vmaxu2(__vmaxu2(most, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu)), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-      }
-      if (__any_sync(0xffffffffu, (most & 0xffffu) >= 0x7f80u || (most >> 16) >= 0x7f80u)) {
-        if (!wait(v_ready + (k & 1), k >> 1)) break;  // group B has read V, and put zeros into its rows past the end
-#pragma unroll 1
-        for (int w = 0; w < kPanel / 256; ++w) {  // word w of this lane's
-          const int i = (w >> 2) * 1024 + (w & 3) * 4;
-          uint32_t* x = reinterpret_cast<uint32_t*>(v + i);
-          const uint32_t keep = ((*x & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((*x & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u);
-          if (keep != 0xffffffffu) {
-            *not_finite = 1;
-            *x &= keep;
-            for (int part = 1; part < kParts; ++part)
-              *reinterpret_cast<uint32_t*>(sm + Lt::kVs + part * kPanel + off + i) &= keep;
-          }
-        }
-        tc::fence_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) tc::mbar_arrive(v_checked + (k & 1));
-    }
   }
   }
   tc::tc_fence_before();
