@@ -241,6 +241,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
         if dv > 1 and v.stride(2) != 1:
             v = v.contiguous()
         ld = _decay(who, log_decay, nh)
+        written = (state,) if out is None else (state, out)
         if out is None:
             out = torch.empty_like(v, memory_format=torch.contiguous_format)
         elif out.shape != (bsz, nh, dv) or out.dtype != q.dtype or (dv > 1 and out.stride(-1) != 1) or any(
@@ -250,4 +251,5 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
                        v.data_ptr(), *v.stride()[:2], out.data_ptr(), *out.stride()[:2], ld.data_ptr(), state.data_ptr(),
                        *at[:3], scale)
         _lib.call("hxm_linear_attn_step", a, stream_of(dev))
+    torch.autograd.graph.increment_version(written)  # gradients that need what was there are refused
     return out

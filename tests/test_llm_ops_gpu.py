@@ -371,3 +371,19 @@ def test_integers_of_every_type(ops, kind):
         m = torch.tensor([-3, 5, 127], device="cuda")
         assert torch.equal(ops.linear_attention(q, k, v, ld, lengths=m.to(kind)), ops.linear_attention(q, k, v, ld, lengths=m.clamp(min=0)))
         assert torch.equal(ops.sample_tokens(x, u, top_k=m.to(kind)), ops.sample_tokens(x, u, top_k=m.clamp(min=0)))
+
+
+def test_a_state_that_autograd_keeps_is_not_changed_behind_its_back(ops):
+    """A step updates its state in place: gradients that need the old state say so, as for any torch operator that
+    writes in place, and so do those that need what `out` held."""
+    q, k, v, ld, s0 = inputs(2, 9, 2, 16, 24, F32, seed=2, s0=True)
+    leaf = q.clone().requires_grad_()
+    for change in (lambda: ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0),
+                   lambda: ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0.clone(), out=v[:, 3])):
+        o = ops.linear_attention(leaf, k, v, ld, initial_state=s0)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(o.sum(), leaf)
+    with torch.inference_mode():
+        s = s0.clone()
+        ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s)
