@@ -80,6 +80,8 @@ def _fill(who, q, k, v, log_decay, scale, lengths, s0, out, sT, error_flag, wait
         if lengths.dtype != torch.int32:
             lengths = lengths.long().clamp(0, L).int()  # widened first: L may be beyond the type's range
         lengths = lengths.contiguous()
+    if error_flag is not None and (error_flag.dtype != torch.int32 or error_flag.numel() < 1):
+        raise ValueError(f"{who}: error_flag must be an int32 tensor with an element, got {error_flag.dtype} {tuple(error_flag.shape)}")
     if s0 is not None:
         if s0.shape != (bsz, nh, dk, v.shape[-1]):
             raise ValueError(f"{who}: initial_state must be {(bsz, nh, dk, v.shape[-1])}, got {tuple(s0.shape)}")

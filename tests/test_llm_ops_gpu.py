@@ -387,3 +387,17 @@ def test_a_state_that_autograd_keeps_is_not_changed_behind_its_back(ops):
     with torch.inference_mode():
         s = s0.clone()
         ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s)
+
+
+def test_error_flags_that_are_no_flags(ops):
+    """error_flag is one 32-bit word that a kernel may write: any other tensor is refused."""
+    q, k, v, ld, _ = inputs(1, 9, 2, 16, 24, F32)
+    for flag in (torch.zeros(1, device="cuda", dtype=torch.uint8), torch.zeros(0, device="cuda", dtype=torch.int32),
+                 torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda", dtype=torch.int64)):
+        with pytest.raises(ValueError, match="error_flag"):
+            ops.linear_attention(q, k, v, ld, error_flag=flag)
+        with pytest.raises(ValueError, match="error_flag"):
+            ops.linear_attention_bwd(q, k, v, ld, v, error_flag=flag)
+    flag = torch.zeros(2, device="cuda", dtype=torch.int32)
+    ops.linear_attention(q, k, v, ld, error_flag=flag)
+    assert int(flag.abs().sum()) == 0
