@@ -193,7 +193,8 @@ struct Ctx {
   const K* keys;
   int n;        // this CTA's tokens
   double max, c;  // weight of x: 2^((x - max) c / kTab); max is finite
-  float fmax, per_bin;  // a bin: 1024 of the latter
+  float fmax, half;  // the largest logit, and half of it
+  float per_bin;     // places in a difference of 2; a bin has 1024
   uint32_t kmax, live;  // of the largest logit; below it no weight
   int flip;
 };
@@ -221,12 +222,13 @@ HXM_DEV u64 to_fixed(double w) { return (u64)__double_as_longlong(w + 4503599627
 template <typename T>
 HXM_DEV u64 weight(const Ctx<T>& c, uint32_t key) { return key >= c.live ? to_fixed(weight_d(c, key)) : 0; }
 
-// Places below the largest logit, in 1/1024 of a bin; the last bin is open.  diff * per_bin + 2^23 ends
-// in the integer; anything larger than the last place (infinity and NaN too) has larger bits.
+// Places below the largest logit, in 1/1024 of a bin; the last bin is open.  diff / 2 * per_bin + 2^23 ends
+// in the integer; anything larger than the last place (NaN too) has larger bits.  (Half of a difference: a whole one
+// may be beyond fp32, and an infinite one lies in the last bin at any temperature.)
 template <typename T>
 HXM_DEV uint32_t place_of(const Ctx<T>& c, uint32_t key) {
   constexpr uint32_t k23 = 0x4b000000u;  // 2^23
-  return min(__float_as_uint(fmaf(c.fmax - Key<T>::value(key), c.per_bin, 8388608.f)), k23 + ((kBins - 1) << 10)) - k23;
+  return min(__float_as_uint(fmaf(fmaf(Key<T>::value(key), -0.5f, c.half), c.per_bin, 8388608.f)), k23 + ((kBins - 1) << 10)) - k23;
 }
 // The smallest key in [1, kmax] for which pass(key) holds; it rises with the key and holds for kmax (a whole
 // warp calls: the 32 keys around a guess, then 33 parts a step).
@@ -249,7 +251,7 @@ HXM_DEV uint32_t first_key(const Ctx<T>& c, float guess, F pass) {
 template <typename T>
 HXM_DEV uint32_t bin_floor(const Ctx<T>& c, int b) {
   if (b < 0) return c.kmax + 1;
-  return first_key(c, c.fmax - (float)((b + 1) << 10) / c.per_bin, [&](uint32_t key) { return (int)(place_of(c, key) >> 10) <= b; });
+  return first_key(c, c.fmax - (float)((b + 1) << 11) / c.per_bin, [&](uint32_t key) { return (int)(place_of(c, key) >> 10) <= b; });
 }
 
 // The keys of kBatch tokens in a row from i on, 0 behind the last one.
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   __shared__ Shared sh;
   unsigned char* region = raw_smem;
   K* keys = reinterpret_cast<K*>(raw_smem + kRegion);
-  Ctx<T> c{cg::this_cluster(), &sh, region, keys, 0, 0, 0, 0.f, 0.f, 0, 0, 0};
+  Ctx<T> c{cg::this_cluster(), &sh, region, keys, 0, 0, 0, 0.f, 0.f, 0.f, 0, 0, 0};
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / c.cl.num_blocks(), rank = c.cl.block_rank();
   int i0 = rank * p.slice;
@@ -738,7 +740,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
   }
   c.max = (double)c.fmax;
   c.c = kTab * 1.4426950408889634074 / (double)temp;
-  c.per_bin = fminf(1024.f * kBinsPerUnit / temp, 3e38f);
+  c.half = 0.5f * c.fmax;
+  c.per_bin = fminf(2048.f * kBinsPerUnit / temp, 3e38f);
   // -45.5 in the exponent of two: weights below it round to 0, and any bound up to -46 would do
   c.live = max(Key<T>::floor_of(__double2float_ru(c.max - 45.5 * 0.69314718055994530942 * (double)temp)), 1u);
   const float u = p.uniforms[row];

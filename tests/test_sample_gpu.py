@@ -253,3 +253,19 @@ def test_settings_of_rows_in_other_types(sample):
         else:
             assert torch.equal(sample(logits, u, temperature=t, top_k=k, top_p=p, min_p=torch.zeros_like(M)),
                                sample(logits, u, temperature=t, top_k=k, top_p=p))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_further_apart_than_the_largest_number(sample, dtype):
+    """Differences of logits beyond the largest fp32 number, at temperatures where such tokens keep weight: they lie at
+    their places among the others."""
+    V = 3000
+    logits, u = make(6, V, dtype, seed=21)
+    big = torch.finfo(torch.bfloat16).max
+    steps = torch.linspace(-1, 1, 9, device="cuda")[torch.randint(0, 9, (6, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))]
+    logits[:3] = (steps[:3] * big).to(dtype)
+    logits[3, 5:9] = big
+    logits[3, 20:900] = -big
+    for T in (1e37, 2e38, float("inf")):
+        for K, P, M in ((0, 0.3, 0.0), (0, 0.9, 0.0), (2000, 1.0, 0.0), (2000, 0.7, 0.0), (30, 0.9, 0.0), (0, 1.0, 0.2)):
+            check(sample, logits, u, T, K, P, M)
