@@ -433,6 +433,7 @@ static hxm_status run(Common c, Problem* p, int np, hxm_dtype io, float* ws, siz
   }
   HXM_REQUIRE(need == 0 || (ws && ws_bytes >= need * sizeof(float)), "%s: workspace %zu bytes < %zu", who, ws_bytes,
               need * sizeof(float));
+  HXM_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(ws) % 16 == 0, "%s: workspace must be 16-byte aligned", who);
   for (int pass = c.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
     if (!tc) {
       const hxm_status s = launch_generic(c, p, np, io, pass == 0, st);

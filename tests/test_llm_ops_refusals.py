@@ -166,3 +166,15 @@ def test_forward_mode_is_refused():
                 go(x)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(lambda t: go(t), (x,), (torch.ones_like(x),))
+
+
+def test_linear_attn_workspace_off_its_alignment():
+    """The segments' sums are read in 16-byte pieces: such a workspace would be a misaligned access."""
+    f = attn(seqlen=100000, heads=1)
+    for n in ("q", "k", "v", "out", "log_decay"):
+        setattr(f, n, 1 << 20)
+    f.struct_size = ct.sizeof(f)
+    f.workspace_bytes = _lib.lib().hxm_linear_attn_workspace_size(f)
+    f.workspace = (1 << 20) + 4
+    got, said = call("hxm_linear_attn_fwd", f)  # refused before the addresses are used
+    assert got == _lib.HXM_EBADARG and "16-byte aligned" in said
