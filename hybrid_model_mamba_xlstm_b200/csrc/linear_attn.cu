@@ -351,7 +351,8 @@ static hxm_status check_args(const hxm_linear_attn_args* a, const char* who) {
   HXM_REQUIRE_SUPPORTED((int64_t)a->batch * 3 <= 65535 && a->heads <= 65535, "%s: batch %d (at most 21845) or heads %d (at most 65535)", who,
                         a->batch, a->heads);
   HXM_REQUIRE_SUPPORTED(a->seqlen <= (1 << 30), "%s: seqlen %d (at most 2^30)", who, a->seqlen);
-  HXM_REQUIRE(a->scale != 0.f && a->scale - a->scale == 0.f, "%s: scale must be finite and nonzero", who);
+  // the gradients divide by it
+  HXM_REQUIRE(fabsf(a->scale) >= 0x1p-126f && fabsf(a->scale) <= 0x1p126f, "%s: scale must be nonzero, of 2^-126 to 2^126", who);
   return HXM_OK;
 }
 

@@ -8,7 +8,6 @@ gate and without input gate and normalizer:
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -39,8 +38,8 @@ def _check(who, q, k, v):
 
 def _scale(who, scale, dk):
     scale = dk ** -0.5 if scale is None else float(scale)
-    if scale == 0 or not math.isfinite(scale) or ctypes.c_float(scale).value == 0:
-        raise ValueError(f"{who}: scale must be finite and nonzero, got {scale}")
+    if not 2.0 ** -126 <= abs(scale) <= 2.0 ** 126:  # the gradients divide by it
+        raise ValueError(f"{who}: scale must be nonzero, of 2^-126 to 2^126, got {scale}")
     return scale
 
 
@@ -183,14 +182,14 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
     q, k (B, L, H, dk), v (B, L, H, dv): bf16 or fp32, any strides (views with a unit last stride and
     16-byte aligned rows are read in place, zero strides too, others copied); log_decay (H,) fp32, at
     most 0 (-inf: each step forgets all before it), a constant without a gradient; scale: default
-    dk**-0.5; lengths (B,) integers: only the first lengths[b] steps of row b count (held to
-    [0, L]), later rows of the output are zero and their inputs are never used; initial_state
-    (B, H, dk, dv).  Returns o (B, L, H, dv) in q's dtype [and the state after the last counted step,
-    fp32 (B, H, dk, dv), to continue with this function or :func:`linear_attention_step`].  An infinity or NaN
-    among the inputs makes what the recurrence forms from it infinite or NaN (which of them is not defined), and
-    nothing else: no earlier step, other head or row.
+    dk**-0.5, of 2^-126 to 2^126 in size; lengths (B,) integers: only the first lengths[b] steps of row b
+    count (held to [0, L]), later rows of the output are zero and their inputs are never used;
+    initial_state (B, H, dk, dv).  Returns o (B, L, H, dv) in q's dtype [and the state after the last counted
+    step, fp32 (B, H, dk, dv), to continue with this function or :func:`linear_attention_step`].  An infinity
+    or NaN among the inputs makes what the recurrence forms from it infinite or NaN (which of them is not
+    defined), and nothing else: no earlier step, other head or row.
 
-    dk <= 512, and dv <= 512 for gradients.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
+    dk <= 512, and dv <= 512 for gradients; B <= 21845, H <= 65535, L <= 2^30.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
     dv <= 256 too) runs on the tensor cores; everything else on the FP32 pipe.  error_flag: a device int32
     tensor set to 1 if a bounded device wait of the call or of its gradients gave up (the outputs are then
     not valid); wait_limit_cycles: that bound in SM cycles (0: about 2 s)."""

@@ -595,7 +595,7 @@ hxm_status hxm_mlstm_gate_epilogue(const hxm_mlstm_gates_args* args, void* strea
 /* with unit stride in the last dim, element strides (b, t, h) given; a zero   */
 /* stride repeats the data along that dim.  log_decay (heads) fp32, <= 0       */
 /* (-inf: no memory).  s0, sT: fp32 with four element strides (b, h, dk, dv).  */
-/* dk <= 512; scale finite and nonzero.  bf16 with dk <= 256, dk and dv        */
+/* dk <= 512; |scale| of 2^-126 to 2^126.  bf16 with dk <= 256, dk and dv      */
 /* multiples of 8 and 16-byte aligned rows runs on the tensor cores.           */
 /* batch <= 21845, heads <= 65535, seqlen <= 2^30; workspace 16-byte aligned.   */
 typedef struct hxm_linear_attn_args {

@@ -178,3 +178,11 @@ def test_linear_attn_workspace_off_its_alignment():
     f.workspace = (1 << 20) + 4
     got, said = call("hxm_linear_attn_fwd", f)  # refused before the addresses are used
     assert got == _lib.HXM_EBADARG and "16-byte aligned" in said
+
+
+@pytest.mark.parametrize("scale", [1e-39, -1e-39, 2e38])
+def test_linear_attn_scales_without_a_reciprocal(scale):
+    got, said = call("hxm_linear_attn_fwd", attn(scale=scale))
+    assert got == _lib.HXM_EBADARG and "scale" in said
+    with pytest.raises(ValueError, match="scale"):
+        kernels.linear_attention(torch.zeros(1, 4, 2, 8), torch.zeros(1, 4, 2, 8), torch.zeros(1, 4, 2, 8), torch.zeros(2), scale=scale)
