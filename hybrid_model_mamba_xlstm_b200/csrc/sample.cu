@@ -17,8 +17,9 @@
 //     pass; so are all keys where the list would not fit (logits of few values);
 //   - the draw: sums of runs of 128 tokens (of which the pass before has most already), the run that holds the
 //     target, the token in it.
-// 256 x 50304 bf16, GPU time: greedy 16 us, top_k 50 25, all tokens 40, top_p 0.9 82; 1 x 50304 fp32: 7, 12,
-// 10 and 22; 32 x 131072 fp32, top_p 0.9: 41.
+// 256 x 50304 bf16, a call among others: greedy 18.6 us, top_k 50 26.8, all tokens 41, top_p 0.9 85 (with cold
+// caches and the profiler's clocks 20, 29, 47 and 92); 1 x 50304 fp32, GPU time: 7, 12, 10 and 22; 32 x 131072 fp32,
+// top_p 0.9: 43.
 //
 // Weights w = exp((logit - max) / temperature) are formed in 64 bits and held as integers of 2^-44:
 // their sums are exact, so no order of additions (atomics, cluster size) changes a result, and a

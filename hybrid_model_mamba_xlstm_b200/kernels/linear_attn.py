@@ -189,10 +189,13 @@ def linear_attention(q, k, v, log_decay, *, scale=None, lengths=None, initial_st
     or NaN among the inputs makes what the recurrence forms from it infinite or NaN (which of them is not
     defined), and nothing else: no earlier step, other head or row.
 
-    dk <= 512, and dv <= 512 for gradients; B <= 21845, H <= 65535, L <= 2^30.  bf16 with dk, dv multiples of 8 and dk <= 256 (for gradients
-    dv <= 256 too) runs on the tensor cores; everything else on the FP32 pipe.  error_flag: a device int32
-    tensor set to 1 if a bounded device wait of the call or of its gradients gave up (the outputs are then
-    not valid); wait_limit_cycles: that bound in SM cycles (0: about 2 s)."""
+    dk <= 512, and dv <= 512 for gradients; B <= 21845, H <= 65535, L <= 2^30. bf16 with dk, dv multiples of 8
+    and dk <= 256 (for gradients dv <= 256 too) runs on the tensor cores, where the weights of q k and the copy
+    of the state that meets q are rounded to bf16 like the inputs (a bf16 result is then off by up to 2^-8 of
+    the sum of absolute values besides its own rounding; states and d_initial_state keep 32 bits); everything
+    else on the FP32 pipe. error_flag: a device int32 tensor set to 1 if a bounded device wait of the call or of
+    its gradients gave up (the outputs are then not valid); wait_limit_cycles: that bound in SM cycles (0: about
+    2 s)."""
     who = "linear_attention"
     if q.dim() != 4:
         raise ValueError(f"{who}: q must be (B, L, H, dk), got {tuple(q.shape)}")

@@ -596,7 +596,9 @@ hxm_status hxm_mlstm_gate_epilogue(const hxm_mlstm_gates_args* args, void* strea
 /* stride repeats the data along that dim.  log_decay (heads) fp32, <= 0       */
 /* (-inf: no memory).  s0, sT: fp32 with four element strides (b, h, dk, dv).  */
 /* dk <= 512; |scale| of 2^-126 to 2^126.  bf16 with dk <= 256, dk and dv      */
-/* multiples of 8 and 16-byte aligned rows runs on the tensor cores.           */
+/* multiples of 8 and 16-byte aligned rows runs on the tensor cores, where the */
+/* weights of q k and the copy of the state that meets q are rounded to bf16   */
+/* like the inputs (the state itself, sT and ds0 keep 32 bits).                */
 /* batch <= 21845, heads <= 65535, seqlen <= 2^30; workspace 16-byte aligned.   */
 typedef struct hxm_linear_attn_args {
   size_t struct_size;
