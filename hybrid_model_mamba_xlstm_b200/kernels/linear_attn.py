@@ -234,7 +234,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, out=None):
     if (dv > 1 and at[3] != 1) or (bsz > 1 and at[0] == 0) or (nh > 1 and at[1] == 0) or (dk > 1 and at[2] == 0):
         raise ValueError(f"{who}: state is updated in place: it needs a unit last stride and no repeated rows")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
-                                    or state.requires_grad):
+                                    or state.requires_grad or (out is not None and out.requires_grad)):
         raise ValueError(f"{who}: has no gradient; use linear_attention, or torch.no_grad()")
     scale = _scale(who, scale, dk)
     with on_device(dev):

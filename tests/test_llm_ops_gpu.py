@@ -401,3 +401,16 @@ def test_error_flags_that_are_no_flags(ops):
     flag = torch.zeros(2, device="cuda", dtype=torch.int32)
     ops.linear_attention(q, k, v, ld, error_flag=flag)
     assert int(flag.abs().sum()) == 0
+
+
+def test_a_step_does_not_write_into_a_graph(ops):
+    """An `out` that autograd has a history or a gradient for is refused, as by torch's own out= functions."""
+    q, k, v, ld, s0 = inputs(2, 1, 2, 16, 24, F32, seed=2, s0=True)
+    before = s0.clone()
+    leaf = torch.zeros(2, 2, 24, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="no gradient"):
+            ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out=out)
+    assert torch.equal(s0, before)
+    with torch.no_grad():
+        ops.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s0, out=leaf)
